@@ -112,6 +112,15 @@ SIGNATURES = {
     "gs_image_loss": (ctypes.c_int, [_P, _I64, _P, _P, _I32, _F, _I32, _P, _P]),
     "gs_adam_step": (ctypes.c_int, [_P, _I32, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.POINTER(_F * 5),
                                     _F, _F, _F, _I32, _I32, _F]),
+    "gs_sh_quantize": (ctypes.c_int, [_P, _I32, _P, _P]),
+    "gs_sh_dequantize": (ctypes.c_int, [_P, _I32, _P, _P]),
+    "gs_sh_color": (ctypes.c_int, [_P, _I32, _P, _P, _I32, _I32, ctypes.POINTER(ctypes.c_double), _P, _P]),
+    "gs_sh_color_backward": (ctypes.c_int, [_P, _I32, _P, _P, _I32, _I32, ctypes.POINTER(ctypes.c_double), _P, _P, _I32, _P,
+                                            _P]),
+    "gs_opacity_dropout": (ctypes.c_int, [_P, _I32, _P, _I32, ctypes.c_double, ctypes.c_uint64, _I32,
+                                          ctypes.POINTER(ctypes.c_uint64), _P]),
+    "gs_opacity_dropout_backward": (ctypes.c_int, [_P, _I32, _P, _I32, ctypes.c_double, ctypes.c_uint64, _I32,
+                                                   ctypes.POINTER(ctypes.c_uint64), _P, _I32, _P]),
     "rasterize_tile": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_int, ctypes.c_int,
                                       ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
 }

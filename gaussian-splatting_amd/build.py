@@ -9,8 +9,12 @@ LIB = os.path.join(HERE, "libgsplat_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -fno-slp-vectorize: SLP packing into v_pk_*_f32 / v_pk_*_f64 costs more issue cycles than the scalar ops it
 # replaces on gfx950 (measured: blend -30 %, K8 -8 %)
-COMMON = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", "-fno-slp-vectorize"]
-# preprocess.hip holds the discontinuous fp64 chain: no FMA contraction there
+# -packed-fp32-ops: no packed fp32 instructions at all, which the compiler also makes from float2 code (the host pass
+# does not know the feature and says so)
+COMMON = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", "-fno-slp-vectorize",
+          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# preprocess.hip holds the discontinuous fp64 chain: no FMA contraction there, nor in the colour product that shares
+# its colour code
 SOURCES = {
     "ctx.hip": [],
     "preprocess.hip": ["-ffp-contract=off"],
@@ -21,6 +25,8 @@ SOURCES = {
     "tile_shim.hip": [],
     "train.hip": [],
     "stats.hip": [],
+    "sh_pack.hip": ["-ffp-contract=off"],
+    "dropout.hip": [],
 }
 
 

@@ -152,7 +152,8 @@ extern "C" int gs_ctx_set_option(gs_ctx *ctx, const char *name, int32_t value) {
 
 static const char *const k_kernel_names[GS_K_NUM] = {
     "preprocess", "bin_count", "bin_scan", "bin_offsets", "bin_duplicate", "bin_sort", "bin_ranges",
-    "blend_forward", "blend_backward", "grad_unpack", "param_backward", "blend_pack", "bin_depth_sort", "image_loss", "adam_step"};
+    "blend_forward", "blend_backward", "grad_unpack", "param_backward", "blend_pack", "bin_depth_sort", "image_loss", "adam_step",
+    "sh_pack", "sh_color", "dropout"};
 
 static hipEvent_t prof_event(gs_ctx *c) {
     if (!c->prof_free.empty()) {

@@ -414,6 +414,50 @@ int gs_adam_step(gs_ctx *ctx, int32_t N, float *means, float *log_scales, float 
                  float *sh, const float *grad_flat, float *m_flat, float *v_flat, const float *lr_host5,
                  float beta1, float beta2, float eps, int32_t step, int32_t mode, float sgd_scale);
 
+/* Packed SH: a gaussian's 48 SH coefficients [3][16] as one 32-byte record, 192 -> 32 bytes (no counterpart in the
+ * reference, which keeps them in full precision).  words[N][8] uint32, as four 64-bit little-endian numbers q0..q3:
+ *   q0       half-precision bits of the constant terms (k = 0) of r, g, b at bits 0, 16, 32; scale bytes of r and g at
+ *            bits 48 and 56
+ *   q1..q3   channel r, g, b: the E2M1 code (sign, two exponent bits, one mantissa bit: 0, .5, 1, 1.5, 2, 3, 4, 6) of
+ *            coefficient k = 1..15 at bit 4 (k - 1); bits 60..63: the low half (r) and the high half (g) of the scale
+ *            byte of b, 0 (b)
+ * Coefficient k of a channel with scale byte s is its code's value times 2^(s - 127).  gs_sh_quantize takes for s the
+ * exponent of the channel's largest magnitude (k >= 1) rounded to one mantissa bit, minus 2, within 0..252, and rounds to
+ * the nearest code, ties to the even one, 6 scales at most; a channel with a NaN or an infinity among k >= 1 becomes NaN
+ * (s = 255).  The constant terms are rounded to half precision (finite values saturate at 65504).
+ * words must be 16-byte aligned, sh too.  gs_sh_dequantize writes the 48 floats a record stands for. */
+int gs_sh_quantize(gs_ctx *ctx, int32_t N, const float *sh, uint32_t *words);
+int gs_sh_dequantize(gs_ctx *ctx, int32_t N, const uint32_t *words, float *sh);
+
+/* View-dependent colour from packed SH, for n_views cameras at once: the colour part of forward_pass (py_compute_color,
+ * forward_pass.py:168-215) of EVERY gaussian (no culling).  cam_pos_host[n_views][3]: HOST doubles, camera_r^T @ camera_t
+ * as forward_pass.py:47 forms them.  colors[n_views][N][3] = max(0, .5 + sum_k Y_k(d) c_k) with d the unit vector from
+ * the camera position to the mean, clamped[n_views][N][3] = 1 where the sum was negative; coefficients above `degree` do
+ * not take part.  Where gs_preprocess does not cull the gaussian, colour and flag equal its results on the dequantised
+ * coefficients bit for bit. */
+int gs_sh_color(gs_ctx *ctx, int32_t N, const uint32_t *words, const float *means, int32_t degree, int32_t n_views,
+                const double *cam_pos_host, float *colors, uint8_t *clamped);
+/* Its gradients, summed over the views (sh_backpass + kernel sh_grads, backward_pass.py:70-97, setup_gpu.py:256-303;
+ * intent): dL_dsh[N][3][16] w.r.t. the coefficients the records stand for (a caller that trains the coefficients the
+ * records were made from takes it for theirs: straight through the rounding), dL_dmeans[N][3] through the direction.
+ * Clamped channels contribute nothing.  Written, or added to when accumulate != 0. */
+int gs_sh_color_backward(gs_ctx *ctx, int32_t N, const uint32_t *words, const float *means, int32_t degree,
+                         int32_t n_views, const double *cam_pos_host, const uint8_t *clamped, const float *dL_dcolors,
+                         int32_t accumulate, float *dL_dsh, float *dL_dmeans);
+
+/* Opacity dropout (no counterpart in the reference): per view, gaussian i is left out with probability p and the opacities
+ * that stay are divided by 1 - p.  out[n_views][N] = keep ? o / (1 - p) : 0 with o = opacity[i], or its sigmoid when
+ * opacity_is_logit != 0.  The mask is not stored: view s (view_ids_host, HOST, any 64-bit numbers) keeps gaussian i iff
+ * word (s & 3) of Philox4x32-10 at the counter (i, 0, low and high 32 bits of s >> 2) under the key `seed` is at least
+ * round(p 2^32), 0 <= p < 1.  gs_opacity_dropout_backward evaluates it again:
+ * dL_dopacity[i] = do/dopacity / (1 - p) * sum over the views that keep i of dL_dout[view][i], written, or added to when
+ * accumulate != 0; gradients of left-out gaussians are not read into the sum, NaN included. */
+int gs_opacity_dropout(gs_ctx *ctx, int32_t N, const float *opacity, int32_t opacity_is_logit, double p, uint64_t seed,
+                       int32_t n_views, const uint64_t *view_ids_host, float *out);
+int gs_opacity_dropout_backward(gs_ctx *ctx, int32_t N, const float *opacity, int32_t opacity_is_logit, double p,
+                                uint64_t seed, int32_t n_views, const uint64_t *view_ids_host, const float *dL_dout,
+                                int32_t accumulate, float *dL_dopacity);
+
 /* The reference's only native symbol (rasterize.c:27-28), kept as a compatibility shim with
  * HOST pointers and `double` conics (defect B7): blends one 16x16 tile on the device through the
  * same kernel as gs_blend_forward (pixel offset +0.5) and copies the chunk back.  Synchronous.

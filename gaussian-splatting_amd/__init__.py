@@ -13,6 +13,6 @@ from .io import (gaussians_from_point_cloud, knn_distances, load_data, load_gaus
 from .functions import (focal_to_fov, get_jacobian_matrix, get_pixel, get_projection_matrix, get_view_matrix,   # noqa: F401
                         inv_sigmoid, sigmoid)
 from .packed_sh import PackedSH, camera_position, quantize_sh, sh_color, sh_color_backward   # noqa: F401
-from .dropout import dropout_opacity, dropout_opacity_backward   # noqa: F401
+from .dropout import OpacityDropout, dropout_opacity, dropout_opacity_backward   # noqa: F401
 from .densify import Densifier   # noqa: F401
 from .train import train_model   # noqa: F401

@@ -229,7 +229,8 @@ def make_camera(camera, camera_r, camera_t, result_size, tile_size, degrees, fla
 
 
 class GaussianSet:
-    """Parameter container with the field names of gaussian.py:31-37 (the live constructor)."""
+    """Parameter container with the field names of gaussian.py:31-37 (the live constructor).  spherical_harmonics may be a
+    PackedSH (quantize_sh) wherever a GaussianSet is taken."""
 
     def __init__(self, centers, shs, scales, rots, opacities, degrees=3):
         self.center = centers
@@ -272,8 +273,36 @@ def _gaussian_tensors(g, device):
     shape = tuple(sh.shape)
     if shape != (N, 3, 16):
         raise ValueError(f"spherical_harmonics must be [N,3,16] (forward_pass.py:172-204), got {shape}")
-    sh = _dev(sh, torch.float32, device, (N, 3, 16))
+    sh = sh.to(device) if _is_packed(sh) else _dev(sh, torch.float32, device, (N, 3, 16))
     return N, means, scales, quats, sh
+
+
+def _is_packed(sh):
+    """A PackedSH (32-byte records) in the place of the [N,3,16] coefficients."""
+    return hasattr(sh, "words")
+
+
+class bound_sh:
+    """The `sh` argument of the parameter kernels on ctx `c` for gaussians first..first+N: a pointer into the coefficients,
+    or, for a PackedSH, NULL while its records are bound to the ctx (gs_ctx_use_packed_sh) -- unbound on the way out, also
+    when the call inside raises."""
+
+    def __init__(self, c, N, sh, first=0):
+        self.c, self.N, self.sh, self.first = c, N, sh, first
+
+    def __enter__(self):
+        if not _is_packed(self.sh):
+            return ctypes.c_void_p(self.sh.data_ptr() + self.first * 192)
+        if self.N:
+            check(self.c.lib.gs_ctx_use_packed_sh(self.c.handle, self.N,
+                                                  ctypes.c_void_p(self.sh.words.data_ptr() + self.first * 32)),
+                  "gs_ctx_use_packed_sh")
+        return ctypes.c_void_p(0)
+
+    def __exit__(self, *exc):
+        if _is_packed(self.sh):
+            self.c.lib.gs_ctx_use_packed_sh(self.c.handle, 0, None)
+        return False
 
 
 # --------------------------------------------------------------------------- forward_pass
@@ -301,10 +330,11 @@ def forward_pass(ctx, queue, program, camera, camera_r, camera_t, gaussians,
     if training:
         extras = [torch.empty((N,) + s, dtype=f32, device=dev)
                   for s in ((6,), (3, 3), (3,), (3,), (6,), (3,))]
-    check(c.lib.gs_preprocess(c.handle, N, _ptr(means), _ptr(scales), _ptr(quats), _ptr(sh),
-                              ctypes.byref(cam), _ptr(centers), _ptr(depths), _ptr(colors), _ptr(conics),
-                              _ptr(clamped), _ptr(tiles_touched), _ptr(radii), *[_ptr(e) for e in extras]),
-          "gs_preprocess")
+    with bound_sh(c, N, sh) as sh_ptr:
+        check(c.lib.gs_preprocess(c.handle, N, _ptr(means), _ptr(scales), _ptr(quats), sh_ptr,
+                                  ctypes.byref(cam), _ptr(centers), _ptr(depths), _ptr(colors), _ptr(conics),
+                                  _ptr(clamped), _ptr(tiles_touched), _ptr(radii), *[_ptr(e) for e in extras]),
+              "gs_preprocess")
     if numpy_mode:
         f64 = np.float64
         out = [_np_out(centers, f64), _np_out(depths, np.int32), _np_out(colors, f64), _np_out(conics, f64),
@@ -761,10 +791,11 @@ def backward_params(c, means, scales, quats, sh, cam, radii, clamped, d_centers_
     if out is None:
         out = (torch.empty((N, 3), dtype=f32, device=dev), torch.empty((N, 3), dtype=f32, device=dev),
                torch.empty((N, 4), dtype=f32, device=dev), torch.empty((N, 3, 16), dtype=f32, device=dev))
-    check(c.lib.gs_backward_params(c.handle, N, _ptr(means), _ptr(scales), _ptr(quats), _ptr(sh),
-                                   ctypes.byref(cam), _ptr(radii), _ptr(clamped), _ptr(d_centers_px),
-                                   _ptr(d_conics), _ptr(d_colors), int(bool(accumulate)), _ptr(out[0]),
-                                   _ptr(out[1]), _ptr(out[2]), _ptr(out[3])), "gs_backward_params")
+    with bound_sh(c, N, sh) as sh_ptr:
+        check(c.lib.gs_backward_params(c.handle, N, _ptr(means), _ptr(scales), _ptr(quats), sh_ptr,
+                                       ctypes.byref(cam), _ptr(radii), _ptr(clamped), _ptr(d_centers_px),
+                                       _ptr(d_conics), _ptr(d_colors), int(bool(accumulate)), _ptr(out[0]),
+                                       _ptr(out[1]), _ptr(out[2]), _ptr(out[3])), "gs_backward_params")
     return out
 
 

@@ -103,6 +103,8 @@ struct gs_ctx {
     int32_t packed_N = -1;
     const float4 *ext_records = nullptr;   // gs_ctx_use_records: caller-owned records replace ctx->packed
     int32_t ext_records_N = -1;
+    const uint4 *packed_sh = nullptr;      // gs_ctx_use_packed_sh: K1 and K8 read these records instead of `sh`
+    int32_t packed_sh_N = -1;
     bool packed_fresh = false;   // gs_bin_fill_culled packed them: the next gs_blend_forward may reuse them
     bool bin_culled = false;     // gs_bin_count_culled produced bin_N / bin_D
     std::vector<hipStream_t> checked_streams;   // streams whose priority has been checked (gs_ctx_set_stream)
@@ -130,6 +132,9 @@ struct gs_prof_scope {
     gs_prof_scope(gs_ctx *c, int kernel);
     ~gs_prof_scope();
 };
+
+// ctx.hip: what K1 and K8 read the SH coefficients from -- the records of gs_ctx_use_packed_sh (*packed = true) or `sh`
+int gs_sh_source(gs_ctx *ctx, const char *who, int32_t N, const float *sh, const void **src, bool *packed);
 
 static inline int gs_div_up(int a, int b) { return (a + b - 1) / b; }
 

@@ -233,6 +233,28 @@ extern "C" int gs_ctx_use_records(gs_ctx *ctx, int32_t N, const float *records) 
     return GS_OK;
 }
 
+extern "C" int gs_ctx_use_packed_sh(gs_ctx *ctx, int32_t N, const uint32_t *words) {
+    GS_REQUIRE(ctx, "gs_ctx_use_packed_sh: ctx is NULL");
+    GS_REQUIRE(((uintptr_t)words & 15) == 0, "gs_ctx_use_packed_sh: the packed records must be 16-byte aligned");
+    GS_REQUIRE(words == nullptr || N >= 0, "gs_ctx_use_packed_sh: N=%d < 0", N);
+    ctx->packed_sh = reinterpret_cast<const uint4 *>(words);
+    ctx->packed_sh_N = words ? N : -1;
+    return GS_OK;
+}
+
+int gs_sh_source(gs_ctx *ctx, const char *who, int32_t N, const float *sh, const void **src, bool *packed) {
+    *packed = ctx->packed_sh != nullptr;
+    if (*packed) {
+        GS_REQUIRE(ctx->packed_sh_N == N, "gs_ctx_use_packed_sh was given N=%d, %s has N=%d", ctx->packed_sh_N, who, N);
+        *src = ctx->packed_sh;
+        return GS_OK;
+    }
+    GS_REQUIRE(sh, "%s: sh is NULL and no packed records are in use", who);
+    GS_REQUIRE(((uintptr_t)sh & 15) == 0, "%s: sh must be 16-byte aligned", who);
+    *src = sh;
+    return GS_OK;
+}
+
 extern "C" int gs_ctx_destroy(gs_ctx *ctx) {
     if (!ctx) return GS_OK;
     (void)hipSetDevice(ctx->device);

@@ -19,6 +19,7 @@
 #include "common.h"
 #include "precam.h"
 #include "sh_grad.h"
+#include "sh_pack.h"
 #include <math.h>
 #include <stdlib.h>
 #include <string.h>
@@ -35,6 +36,7 @@ struct ViewIn {
     const float *d_centers;   // !ROWS: the reference-shaped separate arrays
     const float *d_conics;
     const float *d_colors;
+    float opacity_scale;      // ROWS: d(opacity the view was blended with) / d(activated opacity); 1 without dropout
 };
 
 struct BatchArgs {
@@ -48,10 +50,10 @@ struct BatchArgs {
 // FAST (chosen per launch on the host): every view has SH degree 3 and the strict clip-space centre, so the degree
 // tests of the 48-term sums fold away (a select per term otherwise); same formulas, results equal to fp32 rounding
 // (FMA contraction is on in this file and differs between the two forms).
-template <bool ROWS, bool FAST>
+template <bool ROWS, bool FAST, bool PACKED>
 __global__ __launch_bounds__(256, GS_K8_WAVES) void param_bwd_kernel(
     int N, const float *__restrict__ means, const float *__restrict__ log_scales,
-    const float *__restrict__ quats, const float *__restrict__ sh, const float *__restrict__ opacity,
+    const float *__restrict__ quats, const void *__restrict__ sh, const float *__restrict__ opacity,
     int opacity_is_logit, const BatchArgs args, int accumulate, float *__restrict__ dL_dmeans,
     float *__restrict__ dL_dlog_scales, float *__restrict__ dL_dquats, float *__restrict__ dL_dopacity,
     float *__restrict__ dL_dsh) {
@@ -86,8 +88,14 @@ __global__ __launch_bounds__(256, GS_K8_WAVES) void param_bwd_kernel(
     // (pitch 261 float4: the transposed reads of the gradient write-out below hit distinct banks)
     constexpr int SH_PITCH = 261;
     __shared__ float4 s_sh4[12][SH_PITCH];
-    {
-        const float4 *sh4 = reinterpret_cast<const float4 *>(sh + (size_t)i * 48);
+    if (PACKED) {      // records of gs_ctx_use_packed_sh
+        float c[48];
+        gs_sh_decode(gs_sh_load(reinterpret_cast<const uint4 *>(sh), i), c);
+#pragma unroll
+        for (int vv = 0; vv < 12; vv++)
+            s_sh4[vv][threadIdx.x] = make_float4(c[4 * vv], c[4 * vv + 1], c[4 * vv + 2], c[4 * vv + 3]);
+    } else {
+        const float4 *sh4 = reinterpret_cast<const float4 *>(sh) + (size_t)i * 12;
 #pragma unroll
         for (int vv = 0; vv < 12; vv++) s_sh4[vv][threadIdx.x] = sh4[vv];
     }
@@ -150,7 +158,7 @@ __global__ __launch_bounds__(256, GS_K8_WAVES) void param_bwd_kernel(
 #endif
         if (in.radius <= 0) continue;
         any = true;
-        g_op += in.d_op;
+        g_op = __builtin_fmaf(in.d_op, args.v[v].opacity_scale, g_op);
         const float *in_c = in.c, *in_con = in.con, *in_col = in.col;
 
         // ---- recompute the W rows and cov2d (forward_pass.py:78-86)
@@ -355,6 +363,12 @@ bool bwd_fast(const BatchArgs &a) {
     return true;
 }
 
+template <bool ROWS>
+auto bwd_kernel(const BatchArgs &a, bool packed) {
+    return bwd_fast(a) ? (packed ? param_bwd_kernel<ROWS, true, true> : param_bwd_kernel<ROWS, true, false>)
+                       : (packed ? param_bwd_kernel<ROWS, false, true> : param_bwd_kernel<ROWS, false, false>);
+}
+
 int check_common(gs_ctx *ctx, int32_t N, const gs_camera *cam) {
     GS_REQUIRE(ctx && cam, "gs_backward_params: ctx/cam is NULL");
     GS_REQUIRE(N >= 0, "gs_backward_params: N=%d < 0", N);
@@ -375,11 +389,14 @@ extern "C" int gs_backward_params(gs_ctx *ctx, int32_t N, const float *means, co
     int rc = check_common(ctx, N, cam);
     if (rc) return rc;
     if (N == 0) return GS_OK;
-    GS_REQUIRE(means && log_scales && quats && sh && radii && clamped && dL_dcenters && dL_dconics &&
+    GS_REQUIRE(means && log_scales && quats && radii && clamped && dL_dcenters && dL_dconics &&
                    dL_dcolors && dL_dmeans && dL_dlog_scales && dL_dquats && dL_dsh,
                "gs_backward_params: NULL array argument");
-    GS_REQUIRE(((uintptr_t)sh & 15) == 0 && ((uintptr_t)dL_dsh & 15) == 0,
-               "gs_backward_params: sh and dL_dsh must be 16-byte aligned");
+    GS_REQUIRE(((uintptr_t)dL_dsh & 15) == 0, "gs_backward_params: dL_dsh must be 16-byte aligned");
+    const void *coefs;
+    bool packed;
+    rc = gs_sh_source(ctx, "gs_backward_params", N, sh, &coefs, &packed);
+    if (rc) return rc;
     BatchArgs args;
     memset(&args, 0, sizeof args);
     args.n_views = 1;
@@ -388,9 +405,9 @@ extern "C" int gs_backward_params(gs_ctx *ctx, int32_t N, const float *means, co
     args.v[0].d_centers = dL_dcenters; args.v[0].d_conics = dL_dconics; args.v[0].d_colors = dL_dcolors;
     GS_HIP(hipSetDevice(ctx->device));
     { gs_prof_scope prof_(ctx, GS_K_PARAM_BWD);
-      auto kern = bwd_fast(args) ? param_bwd_kernel<false, true> : param_bwd_kernel<false, false>;
+      auto kern = bwd_kernel<false>(args, packed);
       hipLaunchKernelGGL(kern, dim3(gs_div_up(N, 256)), dim3(256), 0, ctx->stream, N, means,
-                       log_scales, quats, sh, (const float *)nullptr, 0, args, accumulate, dL_dmeans, dL_dlog_scales,
+                       log_scales, quats, coefs, (const float *)nullptr, 0, args, accumulate, dL_dmeans, dL_dlog_scales,
                        dL_dquats, (float *)nullptr, dL_dsh); }
     GS_HIP(hipGetLastError());
     return GS_OK;
@@ -401,14 +418,25 @@ extern "C" int gs_backward_params_batch(gs_ctx *ctx, int32_t N, const float *mea
                                         int32_t opacity_is_logit, int32_t n_views, const gs_view_backward *views,
                                         int32_t accumulate, float *dL_dmeans, float *dL_dlog_scales,
                                         float *dL_dquats, float *dL_dopacity, float *dL_dsh) {
+    return gs_backward_params_batch_scaled(ctx, N, means, log_scales, quats, sh, opacity, opacity_is_logit, n_views, views, nullptr,
+                                           accumulate, dL_dmeans, dL_dlog_scales, dL_dquats, dL_dopacity, dL_dsh);
+}
+
+extern "C" int gs_backward_params_batch_scaled(gs_ctx *ctx, int32_t N, const float *means, const float *log_scales,
+                                               const float *quats, const float *sh, const float *opacity,
+                                               int32_t opacity_is_logit, int32_t n_views, const gs_view_backward *views,
+                                               const float *opacity_scale, int32_t accumulate, float *dL_dmeans,
+                                               float *dL_dlog_scales, float *dL_dquats, float *dL_dopacity, float *dL_dsh) {
     GS_REQUIRE(ctx, "gs_backward_params_batch: ctx is NULL");
     GS_REQUIRE(N >= 0 && n_views >= 0, "gs_backward_params_batch: negative N or n_views");
     GS_REQUIRE(n_views == 0 || views, "gs_backward_params_batch: views is NULL");
     if (N == 0) return GS_OK;
-    GS_REQUIRE(means && log_scales && quats && sh && dL_dmeans && dL_dlog_scales && dL_dquats && dL_dsh,
+    GS_REQUIRE(means && log_scales && quats && dL_dmeans && dL_dlog_scales && dL_dquats && dL_dsh,
                "gs_backward_params_batch: NULL array argument");
-    GS_REQUIRE(((uintptr_t)sh & 15) == 0 && ((uintptr_t)dL_dsh & 15) == 0,
-               "gs_backward_params_batch: sh and dL_dsh must be 16-byte aligned");
+    GS_REQUIRE(((uintptr_t)dL_dsh & 15) == 0, "gs_backward_params_batch: dL_dsh must be 16-byte aligned");
+    const void *coefs;
+    bool packed;
+    if (const int rc = gs_sh_source(ctx, "gs_backward_params_batch", N, sh, &coefs, &packed)) return rc;
     for (int v = 0; v < n_views; v++) {
         int rc = check_common(ctx, N, views[v].cam);
         if (rc) return rc;
@@ -431,11 +459,12 @@ extern "C" int gs_backward_params_batch(gs_ctx *ctx, int32_t N, const float *mea
             const gs_view_backward &src = views[done + v];
             gs_make_precam(src.cam, &args.v[v].cam);
             args.v[v].radii = src.radii; args.v[v].clamped = src.clamped; args.v[v].rows = src.grad_rows;
+            args.v[v].opacity_scale = opacity_scale ? opacity_scale[done + v] : 1.0f;
         }
         { gs_prof_scope prof_(ctx, GS_K_PARAM_BWD);
-          auto kern = bwd_fast(args) ? param_bwd_kernel<true, true> : param_bwd_kernel<true, false>;
+          auto kern = bwd_kernel<true>(args, packed);
           hipLaunchKernelGGL(kern, dim3(gs_div_up(N, 256)), dim3(256), 0, ctx->stream, N, means,
-                           log_scales, quats, sh, opacity, opacity_is_logit, args, (accumulate || done > 0) ? 1 : 0,
+                           log_scales, quats, coefs, opacity, opacity_is_logit, args, (accumulate || done > 0) ? 1 : 0,
                            dL_dmeans, dL_dlog_scales, dL_dquats, dL_dopacity, dL_dsh); }
         GS_HIP(hipGetLastError());
         done += n;

@@ -8,6 +8,7 @@
 #include "common.h"
 #include "precam.h"
 #include "sh_basis.h"
+#include "sh_pack.h"
 #include <math.h>
 #include <stdlib.h>
 
@@ -179,13 +180,20 @@ __device__ __forceinline__ void preprocess_one(const PreCam &cam, double x, doub
     } while (0);
 }
 
+// PACKED: `sh` holds the 32-byte records of gs_ctx_use_packed_sh; they decode to the floats that gs_sh_dequantize
+// writes, so every output equals that of the full-precision form on those bit for bit
+template <bool PACKED>
 __device__ __forceinline__ void load_params(int i, const float *__restrict__ means, const float *__restrict__ log_scales,
-                                            const float *__restrict__ quats, const float *__restrict__ sh, double &x,
+                                            const float *__restrict__ quats, const void *__restrict__ sh, double &x,
                                             double &y, double &z, double (&q)[4], float (&ls)[3], float (&coef)[48]) {
     x = means[3 * i]; y = means[3 * i + 1]; z = means[3 * i + 2];
     for (int k = 0; k < 4; k++) q[k] = quats[4 * i + k];
     for (int k = 0; k < 3; k++) ls[k] = log_scales[3 * i + k];
-    const float4 *sh4 = reinterpret_cast<const float4 *>(sh + (size_t)i * 48);
+    if (PACKED) {
+        gs_sh_decode(gs_sh_load(reinterpret_cast<const uint4 *>(sh), i), coef);
+        return;
+    }
+    const float4 *sh4 = reinterpret_cast<const float4 *>(sh) + (size_t)i * 12;
 #pragma unroll
     for (int v = 0; v < 12; v++) {
         const float4 f = sh4[v];
@@ -213,16 +221,17 @@ __device__ __forceinline__ void store_view(int i, const ViewOut &w, const PreOut
     }
 }
 
+template <bool PACKED>
 __global__ __launch_bounds__(256) void preprocess_kernel(
     int N, const float *__restrict__ means, const float *__restrict__ log_scales,
-    const float *__restrict__ quats, const float *__restrict__ sh, PreCam cam, ViewOut out,
+    const float *__restrict__ quats, const void *__restrict__ sh, PreCam cam, ViewOut out,
     float *__restrict__ Ws, float *__restrict__ Ms, float *__restrict__ Ts, float *__restrict__ cov2d,
     float *__restrict__ cov3d, float *__restrict__ dirs) {
     const int i = blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= N) return;
     double x, y, z, q[4];
     float ls[3], coef[48];
-    load_params(i, means, log_scales, quats, sh, x, y, z, q, ls, coef);
+    load_params<PACKED>(i, means, log_scales, quats, sh, x, y, z, q, ls, coef);
     PreOut o;
     double M[9], Sg[9];
     gaussian_cov(cam.scale_mod, cam.diag_scale, q[0], q[1], q[2], q[3], ls, M, Sg);
@@ -253,20 +262,21 @@ struct PreBatch {
 #else
 #define GS_K1_OCC
 #endif
-template <bool RECORDS, bool FAST>
+template <bool RECORDS, bool FAST, bool PACKED>
 __global__ __launch_bounds__(256) GS_K1_OCC void preprocess_batch_kernel(int N, const float *__restrict__ means,
                                                                const float *__restrict__ log_scales,
                                                                const float *__restrict__ quats,
-                                                               const float *__restrict__ sh,
-                                                               const float *__restrict__ opacities, const PreBatch b) {
+                                                               const void *__restrict__ sh,
+                                                               const float *__restrict__ opacities,
+                                                               size_t opacity_stride, const PreBatch b) {
     const int i = blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= N) return;
     double x, y, z, q[4];
     float ls[3], coef[48];
     // (the SH coefficients as twelve coalesced 1 KiB loads through wave-private LDS instead of twelve loads of 64
     // quarter lines: 0.190 against 0.191 ms per 8 views -- the loads are not what the kernel waits for)
-    load_params(i, means, log_scales, quats, sh, x, y, z, q, ls, coef);
-    const float opac = RECORDS ? opacities[i] : 0.0f;
+    load_params<PACKED>(i, means, log_scales, quats, sh, x, y, z, q, ls, coef);
+    const float opac0 = RECORDS ? opacities[i] : 0.0f;
     // M and Sigma once per gaussian: the host has checked that the views share scale_mod and the scale switch
     double M[9], Sg[9];
     gaussian_cov(b.cam[0].scale_mod, b.cam[0].diag_scale, q[0], q[1], q[2], q[3], ls, M, Sg);
@@ -284,6 +294,8 @@ __global__ __launch_bounds__(256) GS_K1_OCC void preprocess_batch_kernel(int N, 
             reinterpret_cast<int4 *>(w.tiles_touched)[i] = make_int4(o.rect[0], o.rect[1], o.rect[2], o.rect[3]);
 #pragma unroll
             for (int k = 0; k < 3; k++) w.clamped[3 * i + k] = o.cl[k];
+            // (opacity_stride 0: one opacity for every view)
+            const float opac = opacity_stride && v ? opacities[v * opacity_stride + i] : opac0;
             float4 geo, con, rgb;
             gs_make_record(o.cx, o.cy, opac, o.con[0], o.con[1], o.con[2], o.col[0], o.col[1], o.col[2], geo, con, rgb);
             // The wave's 64 records go through wave-private LDS ([quarter][lane], pitch 68 float4: conflict-free both
@@ -321,6 +333,12 @@ bool pre_fast(const PreBatch &b) {
     for (int v = 0; v < b.n_views; v++)
         if (b.cam[v].degree != 3 || b.cam[v].apply_view || !b.cam[v].tile_pow2) return false;
     return true;
+}
+
+template <bool RECORDS>
+auto batch_kernel(const PreBatch &b, bool packed) {
+    return pre_fast(b) ? (packed ? preprocess_batch_kernel<RECORDS, true, true> : preprocess_batch_kernel<RECORDS, true, false>)
+                       : (packed ? preprocess_batch_kernel<RECORDS, false, true> : preprocess_batch_kernel<RECORDS, false, false>);
 }
 
 }  // namespace
@@ -364,17 +382,20 @@ extern "C" int gs_preprocess(gs_ctx *ctx, int32_t N, const float *means, const f
                    cam->cam_height > 0 && cam->fx > 0 && cam->fy > 0,
                "gs_preprocess: invalid camera/frame description");
     if (N == 0) return GS_OK;
-    GS_REQUIRE(means && log_scales && quats && sh && centers && depths && colors && conics &&
+    GS_REQUIRE(means && log_scales && quats && centers && depths && colors && conics &&
                    clamped && tiles_touched && radii,
                "gs_preprocess: NULL array argument");
-    GS_REQUIRE(((uintptr_t)sh & 15) == 0 && ((uintptr_t)tiles_touched & 15) == 0,
-               "gs_preprocess: sh and tiles_touched must be 16-byte aligned");
+    GS_REQUIRE(((uintptr_t)tiles_touched & 15) == 0, "gs_preprocess: tiles_touched must be 16-byte aligned");
+    const void *coefs;
+    bool packed;
+    if (const int rc = gs_sh_source(ctx, "gs_preprocess", N, sh, &coefs, &packed)) return rc;
     PreCam pc;
     gs_make_precam(cam, &pc);
     GS_HIP(hipSetDevice(ctx->device));
     ViewOut vo{centers, colors, conics, depths, tiles_touched, radii, clamped};
-    { gs_prof_scope prof_(ctx, GS_K_PREPROCESS); hipLaunchKernelGGL(preprocess_kernel, dim3(gs_div_up(N, 256)), dim3(256), 0, ctx->stream, N,
-                       means, log_scales, quats, sh, pc, vo, Ws, Ms, Ts, cov2d, cov3d, dirs); }
+    auto kern = packed ? preprocess_kernel<true> : preprocess_kernel<false>;
+    { gs_prof_scope prof_(ctx, GS_K_PREPROCESS); hipLaunchKernelGGL(kern, dim3(gs_div_up(N, 256)), dim3(256), 0, ctx->stream, N,
+                       means, log_scales, quats, coefs, pc, vo, Ws, Ms, Ts, cov2d, cov3d, dirs); }
     GS_HIP(hipGetLastError());
     return GS_OK;
 }
@@ -386,8 +407,10 @@ extern "C" int gs_preprocess_batch(gs_ctx *ctx, int32_t N, const float *means, c
     GS_REQUIRE(N >= 0 && n_views >= 0, "gs_preprocess_batch: negative N or n_views");
     GS_REQUIRE(n_views == 0 || views, "gs_preprocess_batch: views is NULL");
     if (N == 0 || n_views == 0) return GS_OK;
-    GS_REQUIRE(means && log_scales && quats && sh, "gs_preprocess_batch: NULL parameter array");
-    GS_REQUIRE(((uintptr_t)sh & 15) == 0, "gs_preprocess_batch: sh must be 16-byte aligned");
+    GS_REQUIRE(means && log_scales && quats, "gs_preprocess_batch: NULL parameter array");
+    const void *coefs;
+    bool packed;
+    if (const int rc = gs_sh_source(ctx, "gs_preprocess_batch", N, sh, &coefs, &packed)) return rc;
     for (int v = 0; v < n_views; v++) {
         const gs_view_preprocess &w = views[v];
         GS_REQUIRE(w.cam, "gs_preprocess_batch: view %d has no camera", v);
@@ -416,9 +439,9 @@ extern "C" int gs_preprocess_batch(gs_ctx *ctx, int32_t N, const float *means, c
         }
         done += b.n_views;
         { gs_prof_scope prof_(ctx, GS_K_PREPROCESS);
-          auto kern = pre_fast(b) ? preprocess_batch_kernel<false, true> : preprocess_batch_kernel<false, false>;
-          hipLaunchKernelGGL(kern, dim3(gs_div_up(N, 256)), dim3(256), 0, ctx->stream, N, means, log_scales, quats, sh,
-                             (const float *)nullptr, b); }
+          auto kern = batch_kernel<false>(b, packed);
+          hipLaunchKernelGGL(kern, dim3(gs_div_up(N, 256)), dim3(256), 0, ctx->stream, N, means, log_scales, quats, coefs,
+                             (const float *)nullptr, (size_t)0, b); }
         GS_HIP(hipGetLastError());
     }
     return GS_OK;
@@ -427,12 +450,22 @@ extern "C" int gs_preprocess_batch(gs_ctx *ctx, int32_t N, const float *means, c
 extern "C" int gs_preprocess_batch_records(gs_ctx *ctx, int32_t N, const float *means, const float *log_scales,
                                            const float *quats, const float *sh, const float *opacities,
                                            int32_t n_views, const gs_view_records *views) {
+    return gs_preprocess_batch_records_views(ctx, N, means, log_scales, quats, sh, opacities, 0, n_views, views);
+}
+
+extern "C" int gs_preprocess_batch_records_views(gs_ctx *ctx, int32_t N, const float *means, const float *log_scales,
+                                                 const float *quats, const float *sh, const float *opacities,
+                                                 int64_t opacity_stride, int32_t n_views, const gs_view_records *views) {
     GS_REQUIRE(ctx, "gs_preprocess_batch_records: ctx is NULL");
     GS_REQUIRE(N >= 0 && n_views >= 0, "gs_preprocess_batch_records: negative N or n_views");
     GS_REQUIRE(n_views == 0 || views, "gs_preprocess_batch_records: views is NULL");
     if (N == 0 || n_views == 0) return GS_OK;
-    GS_REQUIRE(means && log_scales && quats && sh && opacities, "gs_preprocess_batch_records: NULL parameter array");
-    GS_REQUIRE(((uintptr_t)sh & 15) == 0, "gs_preprocess_batch_records: sh must be 16-byte aligned");
+    GS_REQUIRE(means && log_scales && quats && opacities, "gs_preprocess_batch_records: NULL parameter array");
+    GS_REQUIRE(opacity_stride == 0 || opacity_stride >= N, "gs_preprocess_batch_records_views: opacity_stride %lld is neither 0 "
+               "nor at least N=%d", (long long)opacity_stride, N);
+    const void *coefs;
+    bool packed;
+    if (const int rc = gs_sh_source(ctx, "gs_preprocess_batch_records", N, sh, &coefs, &packed)) return rc;
     for (int v = 0; v < n_views; v++) {
         const gs_view_records &w = views[v];
         GS_REQUIRE(w.cam, "gs_preprocess_batch_records: view %d has no camera", v);
@@ -449,6 +482,7 @@ extern "C" int gs_preprocess_batch_records(gs_ctx *ctx, int32_t N, const float *
     GS_HIP(hipSetDevice(ctx->device));
     for (int done = 0; done < n_views; done += 0) {
         PreBatch b;
+        const float *view_opacities = opacities + (size_t)opacity_stride * done;
         b.n_views = 0;
         while (done + b.n_views < n_views && b.n_views < MAX_PRE_VIEWS) {      // as in gs_preprocess_batch
             const int v = b.n_views;
@@ -461,9 +495,9 @@ extern "C" int gs_preprocess_batch_records(gs_ctx *ctx, int32_t N, const float *
         }
         done += b.n_views;
         { gs_prof_scope prof_(ctx, GS_K_PREPROCESS);
-          auto kern = pre_fast(b) ? preprocess_batch_kernel<true, true> : preprocess_batch_kernel<true, false>;
-          hipLaunchKernelGGL(kern, dim3(gs_div_up(N, 256)), dim3(256), 0, ctx->stream, N, means, log_scales, quats, sh,
-                             opacities, b); }
+          auto kern = batch_kernel<true>(b, packed);
+          hipLaunchKernelGGL(kern, dim3(gs_div_up(N, 256)), dim3(256), 0, ctx->stream, N, means, log_scales, quats, coefs,
+                             view_opacities, (size_t)opacity_stride, b); }
         GS_HIP(hipGetLastError());
     }
     return GS_OK;

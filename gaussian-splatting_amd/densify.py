@@ -17,6 +17,8 @@ from .pipeline import GROUP_WIDTHS, all_reduce_sum, flat_offsets
 class Densifier:
     def __init__(self, pipe, optimizer=None, grad_threshold=0.0002, percent_dense=0.01, scene_extent=None,
                  min_opacity=0.005, split_factor=1.6, seed=0, max_gaussians=None):
+        if pipe.sh is None:
+            raise ValueError("the pipeline has packed SH only: gaussians cannot be cloned or split (PackedSH.dequantize)")
         self.pipe, self.opt = pipe, optimizer
         self.grad_threshold, self.percent_dense = float(grad_threshold), float(percent_dense)
         self.min_opacity, self.split_factor = float(min_opacity), float(split_factor)
@@ -47,6 +49,8 @@ class Densifier:
         k = 0.5 * max(W, H)
         for st in states:
             vis = st["radii"] > 0
+            if st.get("opacity_scale") is not None:        # left out of this view by the opacity dropout
+                vis = vis & (st["opac"] != 0)
             self.grad_accum += torch.where(vis, st["rows"][:, :2].norm(dim=1) * k, torch.zeros_like(self.grad_accum))
             self.denom += vis.to(torch.float32)
 

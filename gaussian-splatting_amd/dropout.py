@@ -5,6 +5,7 @@ the backward pass evaluates it again, and every rank and device gets the same on
 
     op = dropout_opacity(opacity, p, seed, views)             [N] -> [V,N], in front of gpu_rasterize
     d_opacity = dropout_opacity_backward(d_op, opacity, p, seed, views)
+    train_step(pipe, views, targets, grads, dropout=OpacityDropout(p, seed, first_view=step * len(views)))
 
 Arrays may be NumPy (results come back as NumPy, float64) or torch tensors (results stay on the device).  Calls run on
 torch's current stream of the context's device and do not synchronise."""
@@ -36,6 +37,26 @@ def _opacity(opacity, c):
     if len(shape) not in (1, 2) or (len(shape) == 2 and shape[1] != 1):
         raise ValueError(f"opacity must be [N] or [N,1], got {list(shape)}")
     return shape[0], _dev(opacity, torch.float32, c.device, (shape[0],))
+
+
+class OpacityDropout:
+    """Dropout of one training step: probability p, seed, and the number of the step's first view; the step's view k (its
+    position in the whole batch, whichever rank renders it) is number first_view + k.  A training gives every step numbers
+    of its own: step * views_per_step."""
+
+    def __init__(self, p, seed=0, first_view=0):
+        if not 0.0 <= float(p) < 1.0:
+            raise ValueError(f"dropout probability {p} not in [0, 1)")
+        self.p, self.seed, self.first_view = float(p), _seed(seed), int(first_view)
+
+    @property
+    def scale(self):
+        """What the opacities that stay are multiplied by, and the gradient of a view's opacities with them."""
+        return 1.0 / (1.0 - self.p)
+
+    def opacities(self, opacity, numbers, is_logit, ctx=None):
+        """[V,N] opacities of the step's views `numbers`."""
+        return dropout_opacity(opacity, self.p, self.seed, [self.first_view + int(k) for k in numbers], is_logit, ctx)
 
 
 def dropout_opacity(opacity, p, seed, views, is_logit=False, ctx=None):

@@ -19,7 +19,8 @@ import struct
 
 import numpy as np
 
-from .api import GaussianSet
+from .api import GaussianSet, _is_packed
+from .packed_sh import WORDS, PackedSH
 
 SH_C0 = 0.28209479177387814     # forward_pass.py:8
 
@@ -113,7 +114,10 @@ def save_ply(path, gaussians):
     x y z nx ny nz f_dc_0..2 f_rest_0..44 opacity scale_0..2 rot_0..3."""
     xyz = np.asarray(gaussians.center, dtype=np.float32)
     n = len(xyz)
-    sh = np.asarray(gaussians.spherical_harmonics, dtype=np.float32).reshape(n, 3, 16)
+    sh = gaussians.spherical_harmonics
+    if _is_packed(sh):                    # the PLY layout has full-precision coefficients only
+        sh = sh.dequantize().cpu().numpy()
+    sh = np.asarray(sh, dtype=np.float32).reshape(n, 3, 16)
     names = (["x", "y", "z", "nx", "ny", "nz"] + [f"f_dc_{c}" for c in range(3)] +
              [f"f_rest_{k}" for k in range(45)] + ["opacity"] + [f"scale_{k}" for k in range(3)] +
              [f"rot_{k}" for k in range(4)])
@@ -133,20 +137,27 @@ def save_gaussians(file_path, gaussians):
     """gaussian.py:54-56: np.savez with POSITIONAL arrays (arr_0..arr_5 = center, color, sh, scaling,
     rotation, opacity).  `color` is the DC colour ((sh[:, :, 0]) in the [N,3,16] layout): the live
     constructor never sets self.color, so the reference's own save() raises; this keeps its file
-    layout."""
-    sh = np.asarray(gaussians.spherical_harmonics)
+    layout.  Packed SH are stored as their records (arr_2 uint32 [N,8], 32 bytes per gaussian)."""
+    packed = _is_packed(gaussians.spherical_harmonics)
+    sh = gaussians.spherical_harmonics.numpy() if packed else np.asarray(gaussians.spherical_harmonics)
     color = getattr(gaussians, "color", None)
     if color is None:
-        color = sh[:, :, 0]
+        # a record starts with the three constant terms in half precision
+        color = sh.view(np.float16)[:, :3].astype(np.float64) if packed else sh[:, :, 0]
     np.savez(file_path, np.asarray(gaussians.center), np.asarray(color), sh, np.asarray(gaussians.scaling),
              np.asarray(gaussians.rotation), np.asarray(gaussians.opacity))
 
 
 def load_gaussians(file_path, degrees=3):
-    """Inverse of save_gaussians (the reference has no loader for its own checkpoints)."""
+    """Inverse of save_gaussians (the reference has no loader for its own checkpoints).  A checkpoint with packed SH gives
+    a GaussianSet whose spherical_harmonics are a PackedSH."""
     path = file_path if str(file_path).endswith(".npz") else str(file_path) + ".npz"
     with np.load(path, allow_pickle=False) as d:
         center, _color, sh, scaling, rotation, opacity = (d[f"arr_{k}"] for k in range(6))
+    if sh.dtype == np.uint32:
+        if sh.shape != (len(center), WORDS):
+            raise ValueError(f"{path}: packed SH records must be [{len(center)},{WORDS}], found {list(sh.shape)}")
+        sh = PackedSH(sh)
     return GaussianSet(center, sh, scaling, rotation, opacity, degrees)
 
 

@@ -21,18 +21,19 @@ WORDS = 8      # 32-bit words per record
 
 
 class PackedSH:
-    """The packed SH coefficients of N gaussians: `words` [N,8] int32 on the device (layout: include/gsplat.h, "Packed
-    SH").  Stands in the spherical_harmonics slot of a GaussianSet."""
+    """The packed SH coefficients of N gaussians: `words` [N,8], int32 tensor or 32-bit NumPy array (layout:
+    include/gsplat.h, "Packed SH"), moved to the context's device when one is given.  Stands in the spherical_harmonics
+    slot of a GaussianSet.  Calls copy records that are not on their device there every time: move them once (to())."""
 
     def __init__(self, words, ctx=None):
         if not _is_t(words):
             words = np.asarray(words)
             if words.dtype not in (np.dtype(np.int32), np.dtype(np.uint32)):
                 raise ValueError(f"packed SH records are 32-bit words, got {words.dtype}")
-            words = torch.from_numpy(np.ascontiguousarray(words).view(np.int32))
+            words = torch.from_numpy(np.array(words, order="C").view(np.int32))
         if words.dtype != torch.int32 or words.dim() != 2 or words.shape[1] != WORDS:
             raise ValueError(f"packed SH records must be int32 [N,{WORDS}], got {words.dtype} {list(words.shape)}")
-        if words.device.type == "cpu" or ctx is not None:
+        if ctx is not None:
             words = words.to(_ctx(ctx).device)
         self.words = _aligned(words.contiguous())
 
@@ -53,9 +54,10 @@ class PackedSH:
         words = self.words[index]
         if words.dim() != 2:
             raise IndexError("index a PackedSH with a slice, mask or list")
-        part = object.__new__(PackedSH)
-        part.words = _aligned(words.contiguous())
-        return part
+        return PackedSH(words)
+
+    def to(self, device):
+        return self if self.words.device == torch.device(device) else PackedSH(self.words.to(device))
 
     def numpy(self):
         """The records on the host, uint32 [N,8]."""

@@ -15,6 +15,7 @@ import torch
 
 from . import api
 from ._lib import GsViewRecords, GsViewBackward, GsViewPreprocess, check
+from .packed_sh import quantize_sh
 
 GRAD_FLOATS = 59   # 3 mean + 3 log-scale + 4 quaternion + 1 opacity + 48 SH
 
@@ -74,15 +75,29 @@ class View:
 
 
 class SplatPipeline:
-    """Holds the parameters on one device and runs views through the native kernels."""
+    """Holds the parameters on one device and runs views through the native kernels.
+
+    sh_format="mxfp4": views are rendered from packed SH (32-byte records, gs_sh_quantize).  The coefficients in `sh` stay
+    the parameters: every K1 launch packs them as they are then (`packed`), and the gradients K8 forms with respect to the
+    packed values are taken for theirs, so that a scene trained this way looks the same when it is served from its records.
+    A gaussian set whose spherical_harmonics are a PackedSH is served from those: `sh` is None, and there is nothing to
+    train."""
 
     def __init__(self, gaussians, result_size, tile_size=16, background=(0., 0., 0.), pixel_offset=0.5,
-                 opacity_is_logit=True, ctx=None, cull_tiles=True, apply_view=False, diag_scale=False):
+                 opacity_is_logit=True, ctx=None, cull_tiles=True, apply_view=False, diag_scale=False, sh_format=None):
         self.ctx = api._ctx(ctx)
         self.cam_flags = api.camera_flags(apply_view, diag_scale)   # 0 = the reference's quirks Q1/Q4 kept
         self.cull_tiles = bool(cull_tiles)   # gs_bin_*_culled: same images/gradients, about half the list
         dev = self.ctx.device
         self.N, self.means, self.log_scales, self.quats, self.sh = api._gaussian_tensors(gaussians, dev)
+        self.packed = None
+        if api._is_packed(self.sh):
+            self.packed, self.sh = self.sh, None
+        if sh_format not in (None, "fp32", "mxfp4"):
+            raise ValueError(f"sh_format {sh_format!r} must be 'fp32' or 'mxfp4'")
+        if sh_format == "fp32" and self.sh is None:
+            raise ValueError("the gaussians have packed SH only: sh_format 'fp32' needs PackedSH.dequantize()")
+        self.sh_format = "mxfp4" if self.sh is None else (sh_format or "fp32")
         self.opacity = api._dev(gaussians.opacity, torch.float32, dev, (self.N,))
         self.degrees = int(gaussians.degrees)
         self.result_size = [int(result_size[0]), int(result_size[1])]
@@ -132,11 +147,27 @@ class SplatPipeline:
     def allocations(self):
         return sum(c.info("allocations") for c in self.contexts())
 
-    def export(self):
-        """The current parameters as a host GaussianSet (float64 NumPy, the reference's dtypes)."""
+    def export(self, packed=None):
+        """The current parameters as a host GaussianSet (float64 NumPy, the reference's dtypes).  packed=True: with packed
+        SH; False: with [N,3,16] coefficients; None: with coefficients unless the pipeline has records only."""
         f = lambda t: t.detach().cpu().numpy().astype(np.float64)
-        return api.GaussianSet(f(self.means), f(self.sh), f(self.log_scales), f(self.quats), f(self.opacity),
-                               self.degrees)
+        if packed or (packed is None and self.sh is None):
+            sh = (self.packed if self.sh is None else quantize_sh(self.sh, ctx=self.ctx)).to("cpu")
+        else:
+            sh = f(self.packed.dequantize(self.ctx) if self.sh is None else self.sh)
+        return api.GaussianSet(f(self.means), sh, f(self.log_scales), f(self.quats), f(self.opacity), self.degrees)
+
+    def _kept_sh(self, c):
+        """pack_sh without packing again what the last K1 launch packed."""
+        return self.packed if self.packed is not None and len(self.packed) == self.N else self.pack_sh(c)
+
+    def pack_sh(self, ctx=None):
+        """What K1 and K8 take the SH coefficients from: `sh`, or with sh_format "mxfp4" its records, packed here."""
+        if self.sh_format != "mxfp4":
+            return self.sh
+        if self.sh is not None:
+            self.packed = quantize_sh(self.sh, ctx=ctx or self.ctx)
+        return self.packed
 
     # ---- forward ------------------------------------------------------------------------
     def _alloc_pre(self, cam):
@@ -147,15 +178,24 @@ class SplatPipeline:
                     clamped=torch.empty((N, 3), dtype=torch.uint8, device=dev),
                     rect=torch.empty((N, 4), dtype=i32, device=dev), radii=torch.empty((N,), dtype=i32, device=dev))
 
-    def preprocess_batch(self, views, ctx=None, records=None):
+    def preprocess_batch(self, views, ctx=None, records=None, dropout=None, numbers=None, repack=True):
         """K1 for several views in one pass over the parameters; returns one record per view to hand to
         forward(view, pre=...).  records=True (default): gs_preprocess_batch_records
         writes each view's 64-byte blend records instead of centers / colors / conics, so no pack pass
-        runs per view (the per-view arrays are then None)."""
+        runs per view (the per-view arrays are then None).  dropout (OpacityDropout): every view gets opacities of its
+        own; numbers[k] is view k's number in the step (default: its position in `views`).  repack=False: with sh_format
+        "mxfp4", the records of the last K1 launch are those of the unchanged coefficients."""
         c = ctx or self.ctx
         c.sync_stream()
         records = True if records is None else bool(records)   # the blend kernels read records on either list kind
-        opac = torch.sigmoid(self.opacity) if self.opacity_is_logit else self.opacity   # once for the batch
+        if dropout is None:
+            opac = torch.sigmoid(self.opacity) if self.opacity_is_logit else self.opacity   # once for the batch
+        else:
+            opac = dropout.opacities(self.opacity, range(len(views)) if numbers is None else numbers, self.opacity_is_logit, c)
+            if opac.shape[0] != len(views):
+                raise ValueError(f"{opac.shape[0]} view numbers for {len(views)} views")
+        view_opac = lambda k: opac if dropout is None else opac[k]
+        sh = self.pack_sh(c) if repack else self._kept_sh(c)
         cams = [api.make_camera(v.camera, v.camera_r, v.camera_t, self.result_size, self.tile_size, self.degrees,
                                  self.cam_flags)
                 for v in views]
@@ -166,17 +206,22 @@ class SplatPipeline:
                          depths=torch.empty((N,), dtype=i32, device=dev),
                          clamped=torch.empty((N, 3), dtype=torch.uint8, device=dev),
                          rect=torch.empty((N, 4), dtype=i32, device=dev), radii=torch.empty((N,), dtype=i32, device=dev),
-                         opac=opac) for cam in cams]
+                         opac=view_opac(k)) for k, cam in enumerate(cams)]
             arr = (GsViewRecords * max(len(pres), 1))()
             for k, p in enumerate(pres):
                 arr[k].cam = ctypes.pointer(p["cam"])
                 for name, key in (("records", "rec"), ("depths", "depths"), ("clamped", "clamped"),
                                   ("tiles_touched", "rect"), ("radii", "radii")):
                     setattr(arr[k], name, p[key].data_ptr())
-            check(c.lib.gs_preprocess_batch_records(c.handle, self.N, api._ptr(self.means), api._ptr(self.log_scales),
-                                                    api._ptr(self.quats), api._ptr(self.sh), api._ptr(opac), len(pres),
-                                                    arr), "gs_preprocess_batch_records")
-            return pres
+            with api.bound_sh(c, self.N, sh) as sh_ptr:
+                args = (c.handle, self.N, api._ptr(self.means), api._ptr(self.log_scales), api._ptr(self.quats), sh_ptr,
+                        api._ptr(opac))
+                if dropout is None:
+                    check(c.lib.gs_preprocess_batch_records(*args, len(pres), arr), "gs_preprocess_batch_records")
+                else:
+                    check(c.lib.gs_preprocess_batch_records_views(*args, self.N, len(pres), arr),
+                          "gs_preprocess_batch_records_views")
+            return self._with_dropout(pres, dropout)
         pres = [self._alloc_pre(cam) for cam in cams]
         arr = (GsViewPreprocess * max(len(pres), 1))()
         for k, p in enumerate(pres):
@@ -184,10 +229,18 @@ class SplatPipeline:
             for name, key in (("centers", "centers"), ("depths", "depths"), ("colors", "colors"), ("conics", "conics"),
                               ("clamped", "clamped"), ("tiles_touched", "rect"), ("radii", "radii")):
                 setattr(arr[k], name, p[key].data_ptr())
-        check(c.lib.gs_preprocess_batch(c.handle, self.N, api._ptr(self.means), api._ptr(self.log_scales),
-                                        api._ptr(self.quats), api._ptr(self.sh), len(pres), arr), "gs_preprocess_batch")
-        for p in pres:
-            p["opac"] = opac
+        with api.bound_sh(c, self.N, sh) as sh_ptr:
+            check(c.lib.gs_preprocess_batch(c.handle, self.N, api._ptr(self.means), api._ptr(self.log_scales),
+                                            api._ptr(self.quats), sh_ptr, len(pres), arr), "gs_preprocess_batch")
+        for k, p in enumerate(pres):
+            p["opac"] = view_opac(k)
+        return self._with_dropout(pres, dropout)
+
+    @staticmethod
+    def _with_dropout(pres, dropout):
+        if dropout is not None:
+            for p in pres:
+                p["opacity_scale"] = dropout.scale
         return pres
 
     def forward(self, view, want_keys=False, ctx=None, pre=None, loss=None):
@@ -203,11 +256,12 @@ class SplatPipeline:
             pre = self._alloc_pre(api.make_camera(view.camera, view.camera_r, view.camera_t, self.result_size,
                                                   self.tile_size, self.degrees, self.cam_flags))
             null = ctypes.c_void_p(0)
-            check(c.lib.gs_preprocess(c.handle, N, api._ptr(self.means), api._ptr(self.log_scales),
-                                      api._ptr(self.quats), api._ptr(self.sh), ctypes.byref(pre["cam"]),
-                                      api._ptr(pre["centers"]), api._ptr(pre["depths"]), api._ptr(pre["colors"]),
-                                      api._ptr(pre["conics"]), api._ptr(pre["clamped"]), api._ptr(pre["rect"]),
-                                      api._ptr(pre["radii"]), null, null, null, null, null, null), "gs_preprocess")
+            with api.bound_sh(c, N, self.pack_sh(c)) as sh_ptr:
+                check(c.lib.gs_preprocess(c.handle, N, api._ptr(self.means), api._ptr(self.log_scales),
+                                          api._ptr(self.quats), sh_ptr, ctypes.byref(pre["cam"]),
+                                          api._ptr(pre["centers"]), api._ptr(pre["depths"]), api._ptr(pre["colors"]),
+                                          api._ptr(pre["conics"]), api._ptr(pre["clamped"]), api._ptr(pre["rect"]),
+                                          api._ptr(pre["radii"]), null, null, null, null, null, null), "gs_preprocess")
         opac = pre.get("opac")
         if opac is None:
             opac = torch.sigmoid(self.opacity) if self.opacity_is_logit else self.opacity
@@ -253,7 +307,7 @@ class SplatPipeline:
         c.sync_stream()
         state = dict(ctx=c, cam=pre["cam"], depths=pre["depths"], centers=pre["centers"], colors=pre["colors"],
                      conics=pre["conics"], clamped=pre["clamped"], radii=pre["radii"], opac=opac, binning=binning,
-                     rec=pre.get("rec"))
+                     rec=pre.get("rec"), opacity_scale=pre.get("opacity_scale"))
         with _records(c, self.N, pre.get("rec")):
             if loss is None:
                 image, n_contrib, t_final = api.blend_forward(c, pre["centers"], pre["colors"], opac, pre["conics"],
@@ -324,11 +378,16 @@ class SplatPipeline:
             views[k].radii = at(st["radii"], 1).value
             views[k].clamped = at(st["clamped"], 3).value
             views[k].grad_rows = at(st["rows"], 16).value
-        check(c.lib.gs_backward_params_batch(
-            c.handle, g1 - g0, at(self.means, 3), at(self.log_scales, 3), at(self.quats, 4),
-            at(self.sh, 48), at(self.opacity, 1), int(self.opacity_is_logit), len(states), views,
-            int(bool(accumulate)), at(grads.means, 3), at(grads.log_scales, 3), at(grads.quats, 4),
-            at(grads.opacity, 1), at(grads.sh, 48)), "gs_backward_params_batch")
+        with api.bound_sh(c, g1 - g0, self._kept_sh(c), first=g0) as sh_ptr:
+            head = (c.handle, g1 - g0, at(self.means, 3), at(self.log_scales, 3), at(self.quats, 4), sh_ptr,
+                    at(self.opacity, 1), int(self.opacity_is_logit), len(states), views)
+            tail = (int(bool(accumulate)), at(grads.means, 3), at(grads.log_scales, 3), at(grads.quats, 4),
+                    at(grads.opacity, 1), at(grads.sh, 48))
+            if all(st.get("opacity_scale") is None for st in states):
+                check(c.lib.gs_backward_params_batch(*head, *tail), "gs_backward_params_batch")
+            else:      # views blended with dropped-out opacities
+                scale = (ctypes.c_float * len(states))(*[st.get("opacity_scale") or 1.0 for st in states])
+                check(c.lib.gs_backward_params_batch_scaled(*head, scale, *tail), "gs_backward_params_batch_scaled")
         return grads
 
     def backward(self, state, dL_dimage, grads, accumulate=True):
@@ -352,6 +411,8 @@ class Optimizer:
     param -= lr * grad * loss."""
 
     def __init__(self, pipe, learning_rates=None, method="adam", betas=(0.9, 0.999), eps=1e-15):
+        if pipe.sh is None:
+            raise ValueError("the pipeline has packed SH only: there are no coefficients to update (PackedSH.dequantize)")
         lr = dict(REFERENCE_LEARNING_RATES)
         lr.update(learning_rates or {})
         self.pipe, self.method, self.betas, self.eps = pipe, method, betas, float(eps)
@@ -381,7 +442,7 @@ def _loss_and_rows(pipe, image, state, target, loss_kind, scale, loss_out):
     pipe.backward_rows(state, dL)
 
 
-def _render_on_lanes(pipe, views, mine, targets, losses, n_lanes, loss_kind, scale, fused_loss=False):
+def _render_on_lanes(pipe, views, mine, targets, losses, n_lanes, loss_kind, scale, fused_loss=False, dropout=None):
     """Forward, loss gradient and K7 of this rank's views on n_lanes concurrent lanes.  Returns
     (states, done events per view, lanes)."""
     main = pipe.ctx.current_stream()
@@ -392,12 +453,12 @@ def _render_on_lanes(pipe, views, mine, targets, losses, n_lanes, loss_kind, sca
         lanes = pipe.lanes(n_lanes)
     # K1 for the first view of every lane, then (on the main stream, under those views' binning) for the rest
     first = min(n_lanes, len(mine))
-    pres = pipe.preprocess_batch([views[v] for v in mine[:first]])
+    pres = pipe.preprocess_batch([views[v] for v in mine[:first]], dropout=dropout, numbers=mine[:first])
     for _, stream in lanes:
         stream.wait_stream(main)
     pre_ready = None
     if len(mine) > first:
-        pres += pipe.preprocess_batch([views[v] for v in mine[first:]])
+        pres += pipe.preprocess_batch([views[v] for v in mine[first:]], dropout=dropout, numbers=mine[first:], repack=False)
         pre_ready = main.record_event()
     # Two workspaces per lane: the tile count of a lane's next view is launched right behind this
     # view's K6, so its result is on the host long before the lane has finished K7 and the host
@@ -438,7 +499,7 @@ def _render_on_lanes(pipe, views, mine, targets, losses, n_lanes, loss_kind, sca
     return states, done, lanes
 
 
-def _render_prepared(pipe, views, mine, targets, losses, n_lanes, loss_kind, scale, fused_loss=False):
+def _render_prepared(pipe, views, mine, targets, losses, n_lanes, loss_kind, scale, fused_loss=False, dropout=None):
     """The same work as _render_on_lanes with the front half of every view's lists -- count, depth order, scanned
     offsets -- done per BATCH of views on the main stream (gs_bin_prepare_begin / _end: a dozen launches and one host
     wait per batch instead of per view) and only what scales with the number of pairs -- emit, tile sort, ranges
@@ -458,7 +519,8 @@ def _render_prepared(pipe, views, mine, targets, losses, n_lanes, loss_kind, sca
 
     def start(gi):
         ks = groups[gi]
-        for k, p in zip(ks, pipe.preprocess_batch([views[mine[k]] for k in ks])):
+        for k, p in zip(ks, pipe.preprocess_batch([views[mine[k]] for k in ks], dropout=dropout,
+                                                  numbers=[mine[k] for k in ks], repack=gi == 0)):
             pres[k] = p
         toks[gi] = api.bin_prepare_begin(prep[gi % 2], [pres[k] for k in ks], pipe.result_size, pipe.tile_size,
                                          pipe.pixel_offset, pipe.cull_tiles)
@@ -511,14 +573,14 @@ def _render_prepared(pipe, views, mine, targets, losses, n_lanes, loss_kind, sca
     return states, done, lanes
 
 
-def _render_batched(pipe, views, mine, targets, losses, n_lanes, loss_kind, scale, group):
+def _render_batched(pipe, views, mine, targets, losses, n_lanes, loss_kind, scale, group, dropout=None):
     """The same work as _render_on_lanes with the lists of `group` views built per batch of launches on the main
     stream (gs_bin_culled_batch: no per-view host wait, about 20 launches per group instead of 25 per view) and the
     blend kernels of each view on one of n_lanes - 1 side streams, behind its group's event.  One host wait per
     step: the rect-pair bounds that size the lists.  Returns (states, done events per view, lanes)."""
     main = pipe.ctx.current_stream()
     lanes = pipe.lanes(n_lanes - 1) if n_lanes > 1 else [(pipe.ctx, main)]
-    pres = pipe.preprocess_batch([views[v] for v in mine], records=True)
+    pres = pipe.preprocess_batch([views[v] for v in mine], records=True, dropout=dropout, numbers=mine)
     bounds = []
     for g0 in range(0, len(pres), 8):
         bounds += api.bin_bounds_batch(pipe.ctx, pres[g0:g0 + 8], pipe.result_size, pipe.tile_size)
@@ -598,7 +660,7 @@ def auto_lanes(pipe):
 
 def train_step(pipe, views, targets, grads, loss_scale=None, concurrent_views=2, loss_kind="l2", states_hook=None,
                k8_early_lanes=None, allreduce_chunks=4, batch_binning=False, bin_group=4, prepared=False,
-               fused_loss=False):
+               fused_loss=False, dropout=None):
     """Forward+backward over this rank's shard of `views`, then the all-reduce of the flat gradient
     buffer when torch.distributed is initialised.  targets[v] is the image [W,H,3] view v should
     match; the loss is the mean squared ("l2") or mean absolute ("l1") error summed over the views,
@@ -622,6 +684,8 @@ def train_step(pipe, views, targets, grads, loss_scale=None, concurrent_views=2,
     and two launches per view less; False (default): the separate gs_image_loss pass.  Measured on MI355X at 1 M /
     1080p / 8 views: 5.91 ms fused against 5.82 ms -- the epilogue's 12-byte-per-lane target reads and dL stores are
     worse streams than the loss kernel's float4s, and that outweighs the saved pass.
+    dropout (OpacityDropout): view v of the batch leaves out the gaussians that its number first_view + v says, on whichever
+    rank renders it.
     Returns (sum of local losses as a device scalar, number of local views)."""
     import torch.distributed as dist
     distributed = dist.is_available() and dist.is_initialized()
@@ -641,7 +705,7 @@ def train_step(pipe, views, targets, grads, loss_scale=None, concurrent_views=2,
     if batch_binning and pipe.cull_tiles and len(mine) > 0:
         main = pipe.ctx.current_stream()
         group = max(1, min(int(bin_group), 8))
-        states, done, lanes = _render_batched(pipe, views, mine, targets, losses, n_lanes, loss_kind, scale, group)
+        states, done, lanes = _render_batched(pipe, views, mine, targets, losses, n_lanes, loss_kind, scale, group, dropout)
         # the views of all groups but the last get their parameter backward on the main stream (idle once the
         # lists are built) while the last group still blends
         n_early = (len(mine) - 1) // group * group
@@ -656,7 +720,7 @@ def train_step(pipe, views, targets, grads, loss_scale=None, concurrent_views=2,
     elif n_lanes > 1:
         main = pipe.ctx.current_stream()
         render = _render_prepared if prepared else _render_on_lanes
-        states, done, lanes = render(pipe, views, mine, targets, losses, n_lanes, loss_kind, scale, fused_loss)
+        states, done, lanes = render(pipe, views, mine, targets, losses, n_lanes, loss_kind, scale, fused_loss, dropout)
         # The lanes do not finish together (the hardware serves the queues in a fixed order): K8 of the
         # early lanes' views runs on lane 0's stream while the others still blend.
         if k8_early_lanes is None:
@@ -672,7 +736,7 @@ def train_step(pipe, views, targets, grads, loss_scale=None, concurrent_views=2,
         for _, stream in lanes:
             main.wait_stream(stream)
     else:
-        pres = pipe.preprocess_batch([views[v] for v in mine])
+        pres = pipe.preprocess_batch([views[v] for v in mine], dropout=dropout, numbers=mine)
         for k, v in enumerate(mine):
             la = (targets[v], loss_kind, scale, losses[k:k + 1]) if fused_loss else None
             image, state = pipe.forward(views[v], pre=pres[k], loss=la)

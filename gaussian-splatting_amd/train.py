@@ -19,6 +19,7 @@ import numpy as np
 import torch
 
 from . import io as gio
+from .dropout import OpacityDropout
 from .pipeline import FlatGrads, Optimizer, SplatPipeline, View, all_reduce_sum, train_step
 
 
@@ -39,7 +40,7 @@ def train_model(cameras, images, point_cloud_data, learning_rates, ctx=None, que
                 image_dir="./input/images", output_dir="output/test_run", method="adam", loss="l1",
                 subset_fraction=.2, seed=None, gaussians=None, save_images_every=50, checkpoint_every=100,
                 concurrent_views=4, log=print, densify_every=None, densify_from=500, densify_until=15000,
-                densify_options=None):
+                densify_options=None, drop_rate=0.0, sh_format=None):
     """train.py:12-64.  cameras / images / point_cloud_data: a COLMAP model (io.read_model or the
     reference's reader); learning_rates: the dict of main.py:11-17 (keys center, scaling, opacity,
     rotation, sh).  densify_every=k runs the Densifier (clone / split / prune; no reference
@@ -63,7 +64,7 @@ def train_model(cameras, images, point_cloud_data, learning_rates, ctx=None, que
 
     # the reference keeps raw opacities on the training path (train.py:37) and logits on the PLY
     # path (gaussian.py:50); point-cloud initialisation stores the raw value .1
-    pipe = SplatPipeline(gaussians, result_size, opacity_is_logit=False, ctx=ctx)
+    pipe = SplatPipeline(gaussians, result_size, opacity_is_logit=False, ctx=ctx, sh_format=sh_format)
     dev = pipe.ctx.device
     grads = FlatGrads(pipe.N, dev)
     opt = Optimizer(pipe, learning_rates, method=method)
@@ -71,6 +72,8 @@ def train_model(cameras, images, point_cloud_data, learning_rates, ctx=None, que
     if densify_every:
         from .densify import Densifier
         den = Densifier(pipe, opt, seed=0 if seed is None else seed, **(densify_options or {}))
+    # the masks depend on the seed, the iteration and the view's place in the batch alone: the same on every rank
+    drop_seed = random.SystemRandom().randrange(2 ** 63) if seed is None else int(seed) % 2 ** 64
     target_cache = {}
     history = []
     log("setup complete in {time}s".format(time=time.perf_counter() - t0))
@@ -87,9 +90,11 @@ def train_model(cameras, images, point_cloud_data, learning_rates, ctx=None, que
             if src.id not in target_cache:
                 target_cache[src.id] = torch.from_numpy(np.ascontiguousarray(loader(src), dtype=np.float32)).to(dev)
             targets.append(target_cache[src.id])
+        rate = float(drop_rate(i) if callable(drop_rate) else drop_rate)
+        dropout = OpacityDropout(rate, drop_seed, first_view=i * views_per_step) if rate != 0.0 else None
         loss_sum, n_local = train_step(pipe, views, targets, grads, loss_scale=1.0 / views_per_step,
                                        concurrent_views=concurrent_views, loss_kind=loss,
-                                       states_hook=den.accumulate if den else None)
+                                       states_hook=den.accumulate if den else None, dropout=dropout)
         if distributed:
             # the replicated parameters stay in lock-step only if every rank applies the same update:
             # method="reference" scales it by the loss, so the loss is the mean over the WHOLE batch
@@ -114,4 +119,6 @@ def train_model(cameras, images, point_cloud_data, learning_rates, ctx=None, que
             PILImage.fromarray(pic).save(os.path.join(output_dir, "pass_{iter}.jpg".format(iter=i)))
         if output_dir and checkpoint_every and i % checkpoint_every == 0:         # train.py:63-64
             gio.save_gaussians(os.path.join(output_dir, "iter_{iter}_gaus".format(iter=i)), pipe.export())
+            if pipe.sh_format == "mxfp4":
+                gio.save_gaussians(os.path.join(output_dir, "iter_{iter}_packed".format(iter=i)), pipe.export(packed=True))
     return pipe.export(), history

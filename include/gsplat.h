@@ -445,6 +445,30 @@ int gs_sh_color_backward(gs_ctx *ctx, int32_t N, const uint32_t *words, const fl
                          int32_t n_views, const double *cam_pos_host, const uint8_t *clamped, const float *dL_dcolors,
                          int32_t accumulate, float *dL_dsh, float *dL_dmeans);
 
+/* Makes the parameter kernels read the SH coefficients from packed records: while words != NULL, gs_preprocess*,
+ * gs_preprocess_batch*, gs_backward_params* and gs_backward_params_batch* on this ctx take the coefficients of their N
+ * gaussians from words[N][8] and ignore their `sh` argument (which may be NULL); their outputs are those of the same call
+ * on the dequantised coefficients, bit for bit (gradients to fp32 rounding).  N must be the N of those calls.
+ * gs_ctx_use_packed_sh(ctx, 0, NULL) returns to the argument.  The records must stay unchanged while calls that use them
+ * are in flight. */
+int gs_ctx_use_packed_sh(gs_ctx *ctx, int32_t N, const uint32_t *words);
+
+/* gs_preprocess_batch_records with opacities of its own per view: view v's records are built from
+ * opacities[v * opacity_stride + i] (opacity_stride >= N, the layout gs_opacity_dropout writes; 0: one array for every
+ * view). */
+int gs_preprocess_batch_records_views(gs_ctx *ctx, int32_t N, const float *means, const float *log_scales,
+                                      const float *quats, const float *sh, const float *opacities,
+                                      int64_t opacity_stride, int32_t n_views, const gs_view_records *views);
+
+/* gs_backward_params_batch for views that were blended with dropped-out opacities: the opacity gradient of view v is
+ * multiplied by opacity_scale_host[v] (HOST, 1 / (1 - p); NULL: 1 for every view).  That is the whole backward pass of the
+ * dropout: a gaussian that was left out has opacity 0, reaches alpha 1/255 nowhere, and its gradient row is zero. */
+int gs_backward_params_batch_scaled(gs_ctx *ctx, int32_t N, const float *means, const float *log_scales,
+                                    const float *quats, const float *sh, const float *opacity,
+                                    int32_t opacity_is_logit, int32_t n_views, const gs_view_backward *views,
+                                    const float *opacity_scale_host, int32_t accumulate, float *dL_dmeans,
+                                    float *dL_dlog_scales, float *dL_dquats, float *dL_dopacity, float *dL_dsh);
+
 /* Opacity dropout (no counterpart in the reference): per view, gaussian i is left out with probability p and the opacities
  * that stay are divided by 1 - p.  out[n_views][N] = keep ? o / (1 - p) : 0 with o = opacity[i], or its sigmoid when
  * opacity_is_logit != 0.  The mask is not stored: view s (view_ids_host, HOST, any 64-bit numbers) keeps gaussian i iff

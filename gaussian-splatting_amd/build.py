@@ -13,8 +13,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # does not know the feature and says so)
 COMMON = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", "-fno-slp-vectorize",
           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-# preprocess.hip holds the discontinuous fp64 chain: no FMA contraction there, nor in the colour product that shares
-# its colour code
+# preprocess.hip holds the discontinuous fp64 chain: no FMA contraction there
 SOURCES = {
     "ctx.hip": [],
     "preprocess.hip": ["-ffp-contract=off"],
@@ -25,7 +24,7 @@ SOURCES = {
     "tile_shim.hip": [],
     "train.hip": [],
     "stats.hip": [],
-    "sh_pack.hip": ["-ffp-contract=off"],
+    "sh_pack.hip": [],
     "dropout.hip": [],
 }
 

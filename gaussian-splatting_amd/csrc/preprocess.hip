@@ -7,7 +7,6 @@
 // compiled with -ffp-contract=off so no FMA contraction changes those roundings.
 #include "common.h"
 #include "precam.h"
-#include "sh_basis.h"
 #include "sh_pack.h"
 #include <math.h>
 #include <stdlib.h>
@@ -170,13 +169,48 @@ __device__ __forceinline__ void preprocess_one(const PreCam &cam, double x, doub
 
         // :127 -> py_compute_color (:168-215)
         double dx = x - cam.cam_pos[0], dy = y - cam.cam_pos[1], dz = z - cam.cam_pos[2];
-        // one division and three products for the direction
+        // The colour is a float output (tolerance, not bits; the reference's own sums associate differently, :178-203):
+        // one division and three products for the direction, fused multiply-adds for the 48-term sums.
         const double dn_inv = 1.0 / sqrt((dx * dx + dy * dy) + dz * dz);
         dx *= dn_inv; dy *= dn_inv; dz *= dn_inv;
         if (EXTRAS) { o.eD[0] = dx; o.eD[1] = dy; o.eD[2] = dz; }
         double basis[16];
-        gs_sh_basis(degree, dx, dy, dz, basis);
-        gs_sh_channels(degree, basis, coef, o.col, o.cl);
+        basis[0] = SH_C0;
+        if (degree > 0) {
+            basis[1] = -dy * SH_C1; basis[2] = dz * SH_C1; basis[3] = -dx * SH_C1;
+            if (degree > 1) {
+                const double xx = dx * dx, yy = dy * dy, zz = dz * dz, xy = dx * dy, yz = dy * dz, xz = dx * dz;
+                basis[4] = SH_C2_0 * xy; basis[5] = SH_C2_1 * yz;
+                basis[6] = SH_C2_2 * (2.0 * zz - xx - yy);
+                basis[7] = SH_C2_3 * xz; basis[8] = SH_C2_4 * (xx - yy);
+                if (degree > 2) {
+                    basis[9] = SH_C3_0 * dy * (3.0 * xx - yy);
+                    basis[10] = SH_C3_1 * xy * dz;
+                    basis[11] = SH_C3_2 * dy * (4.0 * zz - xx - yy);
+                    basis[12] = SH_C3_3 * dz * (2.0 * zz - 3.0 * xx - 3.0 * yy);
+                    basis[13] = SH_C3_4 * dx * (4.0 * zz - xx - yy);
+                    basis[14] = SH_C3_5 * dz * (xx - yy);
+                    basis[15] = SH_C3_6 * dx * (xx - 3.0 * yy);
+                }
+            }
+        }
+        const int nb = (degree + 1) * (degree + 1);
+#pragma unroll
+        for (int ch = 0; ch < 3; ch++) {
+            double r = 0.0;
+#pragma unroll
+            for (int k = 0; k < 16; k++)
+                if (k < nb) {
+                    float cf = coef[16 * ch + k];
+#ifdef GS_K1_CVT_IN_LOOP
+                    asm volatile("" : "+v"(cf));        // keep the coefficient a float across views (48 VGPRs, not 96)
+#endif
+                    r = __builtin_fma(basis[k], (double)cf, r);
+                }
+            r += .5;
+            if (r < 0) { r = 0; o.cl[ch] = 1; }
+            o.col[ch] = (float)r;
+        }
     } while (0);
 }
 

@@ -6,8 +6,7 @@
 // All four kernels are bound by HBM: per gaussian 192 + 32 bytes (conversions), 44 + 15 V (colour of V views),
 // 44 + 15 V + 204 (its gradients).  One thread per gaussian.
 #include "common.h"
-#include "sh_basis.h"
-#include "sh_grad.h"
+#include "precam.h"
 #include "sh_pack.h"
 
 namespace {
@@ -65,9 +64,51 @@ __global__ __launch_bounds__(256) void sh_dequantize_kernel(int N, const uint4 *
     for (int v = 0; v < 12; v++) sh[(size_t)i * 12 + v] = make_float4(c[4 * v], c[4 * v + 1], c[4 * v + 2], c[4 * v + 3]);
 }
 
+// ---- colour.  On the unit sphere the 16 basis functions are constants times these polynomials (x^2 + y^2 + z^2 = 1 turns
+// 2zz - xx - yy into 3zz - 1 and so on); the signs are in the constants.
+//   m0..3   1, y, z, x           m4..8  xy, yz, 3zz - 1, xz, xx - yy
+//   m9..15  y (3xx - yy), xyz, y (5zz - 1), z (5zz - 3), x (5zz - 1), z (xx - yy), x (xx - 3yy)
+__device__ constexpr double BASIS_CONST[16] = {SH_C0, -SH_C1, SH_C1, -SH_C1, SH_C2_0, SH_C2_1, SH_C2_2, SH_C2_3, SH_C2_4,
+                                               SH_C3_0, SH_C3_1, SH_C3_2, SH_C3_3, SH_C3_4, SH_C3_5, SH_C3_6};
+
+template <int DEGREE, typename T>
+__device__ __forceinline__ void basis_polynomials(T x, T y, T z, T (&m)[16]) {
+    m[0] = 1;
+    if (DEGREE > 0) { m[1] = y; m[2] = z; m[3] = x; }
+    if (DEGREE > 1) {
+        const T xx = x * x, yy = y * y, zz = z * z;
+        m[4] = x * y; m[5] = y * z; m[6] = 3 * zz - 1; m[7] = x * z; m[8] = xx - yy;
+        if (DEGREE > 2) {
+            const T q = 5 * zz - 1;
+            m[9] = y * (3 * xx - yy); m[10] = m[4] * z; m[11] = y * q; m[12] = z * (q - 2); m[13] = x * q;
+            m[14] = z * m[8]; m[15] = x * (xx - 3 * yy);
+        }
+    }
+}
+
+// 1 / sqrt(x) to the last bits of fp64: the hardware's 24-bit estimate and one step of third order
+__device__ __forceinline__ double inverse_sqrt(double x) {
+    const double y = __builtin_amdgcn_rsq(x);
+    const double e = __builtin_fma(-x * y, y, 1.0);
+    return __builtin_fma(y * e, __builtin_fma(0.375, e, 0.5), y);
+}
+
+struct Direction {
+    double x, y, z, inv;      // unit vector from the camera, 1 / distance
+};
+__device__ __forceinline__ Direction direction(double x, double y, double z, const double (&cam)[3]) {
+    Direction d{x - cam[0], y - cam[1], z - cam[2], 0};
+    d.inv = inverse_sqrt(__builtin_fma(d.x, d.x, __builtin_fma(d.y, d.y, d.z * d.z)));
+    d.x *= d.inv; d.y *= d.inv; d.z *= d.inv;
+    return d;
+}
+
+// In fp64 from the difference of the positions on, as K1 evaluates colours: the flag is the sign of the sum.
+template <int DEGREE>
 __global__ __launch_bounds__(256) void sh_color_kernel(int N, const uint4 *__restrict__ words, const float *__restrict__ means,
-                                                       int degree, const Cameras cams, float *__restrict__ colors,
+                                                       const Cameras cams, float *__restrict__ colors,
                                                        uint8_t *__restrict__ clamped) {
+    constexpr int NB = (DEGREE + 1) * (DEGREE + 1);
     const uint32_t i = blockIdx.x * 256u + threadIdx.x;
     if (i >= (uint32_t)N) return;
     float coef[48];
@@ -75,62 +116,82 @@ __global__ __launch_bounds__(256) void sh_color_kernel(int N, const uint4 *__res
     const double x = means[3 * (size_t)i], y = means[3 * (size_t)i + 1], z = means[3 * (size_t)i + 2];
 #pragma unroll 1
     for (int v = 0; v < cams.n; v++) {
-        double dx = x - cams.pos[v][0], dy = y - cams.pos[v][1], dz = z - cams.pos[v][2];
-        const double inv = 1.0 / sqrt((dx * dx + dy * dy) + dz * dz);
-        dx *= inv; dy *= inv; dz *= inv;
-        double basis[16];
-        gs_sh_basis(degree, dx, dy, dz, basis);
-        float col[3];
-        uint8_t cl[3] = {0, 0, 0};
-        gs_sh_channels(degree, basis, coef, col, cl);
+        const Direction d = direction(x, y, z, cams.pos[v]);
+        double m[16];
+        basis_polynomials<DEGREE, double>(d.x, d.y, d.z, m);
+#pragma unroll
+        for (int k = 0; k < NB; k++) m[k] *= BASIS_CONST[k];
         const size_t o = 3 * ((size_t)v * N + i);
 #pragma unroll
-        for (int ch = 0; ch < 3; ch++) { colors[o + ch] = col[ch]; clamped[o + ch] = cl[ch]; }
+        for (int ch = 0; ch < 3; ch++) {
+            double r = 0.5;
+#pragma unroll
+            for (int k = 0; k < NB; k++) r = __builtin_fma(m[k], (double)coef[16 * ch + k], r);
+            const bool c = r < 0;
+            colors[o + ch] = c ? 0.0f : (float)r;
+            clamped[o + ch] = c;
+        }
     }
 }
 
+// fp32 behind the fp64 direction, as in K8: products and sums of a few dozen terms.  The constants of the basis are taken
+// out of the view loop: they are multiplied into the coefficients in front of it and into the sums behind it.
+template <int DEGREE>
 __global__ __launch_bounds__(256) void sh_color_backward_kernel(int N, const uint4 *__restrict__ words,
-                                                                const float *__restrict__ means, int degree,
-                                                                const Cameras cams, const uint8_t *__restrict__ clamped,
+                                                                const float *__restrict__ means, const Cameras cams,
+                                                                const uint8_t *__restrict__ clamped,
                                                                 const float *__restrict__ d_colors, int accumulate,
                                                                 float4 *__restrict__ d_sh, float *__restrict__ d_means) {
+    constexpr int NB = (DEGREE + 1) * (DEGREE + 1);
     const uint32_t i = blockIdx.x * 256u + threadIdx.x;
     if (i >= (uint32_t)N) return;
     float coef[48], acc[48];
     gs_sh_decode(gs_sh_load(words, i), coef);
 #pragma unroll
-    for (int k = 0; k < 48; k++) acc[k] = 0.0f;
+    for (int k = 0; k < 48; k++) {
+        coef[k] *= (float)BASIS_CONST[k & 15];
+        acc[k] = 0.0f;
+    }
     const double x = means[3 * (size_t)i], y = means[3 * (size_t)i + 1], z = means[3 * (size_t)i + 2];
     double g_mean[3] = {0, 0, 0};
 #pragma unroll 1
     for (int v = 0; v < cams.n; v++) {
-        double dx = x - cams.pos[v][0], dy = y - cams.pos[v][1], dz = z - cams.pos[v][2];
-        const double inv = 1.0 / sqrt((dx * dx + dy * dy) + dz * dz);
-        dx *= inv; dy *= inv; dz *= inv;
-        float basis[16], bx[16], by[16], bz[16], g[3];
-        gs_sh_basis_grad(degree, (float)dx, (float)dy, (float)dz, basis, bx, by, bz);
+        const Direction d = direction(x, y, z, cams.pos[v]);
+        const float dx = (float)d.x, dy = (float)d.y, dz = (float)d.z;
+        float m[16], w[16], g[3];
+        basis_polynomials<DEGREE, float>(dx, dy, dz, m);
         const size_t o = 3 * ((size_t)v * N + i);
 #pragma unroll
         for (int ch = 0; ch < 3; ch++) g[ch] = clamped[o + ch] ? 0.0f : d_colors[o + ch];
-        // w_k = sum over the channels of gradient x coefficient; dL/d(direction) = sum_k w_k grad Y_k
-        const int nb = (degree + 1) * (degree + 1);
-        float ex = 0.0f, ey = 0.0f, ez = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 16; k++)
-            if (k < nb) {
-                const float w = __builtin_fmaf(g[2], coef[32 + k], __builtin_fmaf(g[1], coef[16 + k], g[0] * coef[k]));
-                ex = __builtin_fmaf(bx[k], w, ex);
-                ey = __builtin_fmaf(by[k], w, ey);
-                ez = __builtin_fmaf(bz[k], w, ez);
+        for (int k = 0; k < NB; k++) {
+            w[k] = __builtin_fmaf(g[2], coef[32 + k], __builtin_fmaf(g[1], coef[16 + k], g[0] * coef[k]));
 #pragma unroll
-                for (int ch = 0; ch < 3; ch++) acc[16 * ch + k] = __builtin_fmaf(g[ch], basis[k], acc[16 * ch + k]);
-            }
-        // d = v / |v|: dL/dv = (dL/dd - d (d . dL/dd)) / |v|
-        const double dot = dx * ex + dy * ey + dz * ez;
-        g_mean[0] += ((double)ex - dx * dot) * inv;
-        g_mean[1] += ((double)ey - dy * dot) * inv;
-        g_mean[2] += ((double)ez - dz * dot) * inv;
+            for (int ch = 0; ch < 3; ch++) acc[16 * ch + k] = __builtin_fmaf(g[ch], m[k], acc[16 * ch + k]);
+        }
+        if (DEGREE == 0) continue;
+        // e = sum_k w_k grad m_k.  The polynomials agree with the basis on the sphere only; the component along d, where
+        // they differ, is projected out below.
+        float ex = w[3], ey = w[1], ez = w[2];
+        if (DEGREE > 1) {
+            ex += dy * w[4] + dz * w[7] + 2 * dx * w[8];
+            ey += dx * w[4] + dz * w[5] - 2 * dy * w[8];
+            ez += dy * w[5] + 6 * dz * w[6] + dx * w[7];
+        }
+        if (DEGREE > 2) {
+            const float q = 5 * dz * dz - 1, xy6 = 6 * m[4], xxyy3 = 3 * m[8];
+            ex += xy6 * w[9] + m[5] * w[10] + q * w[13] + 2 * m[7] * w[14] + xxyy3 * w[15];
+            ey += xxyy3 * w[9] + m[7] * w[10] + q * w[11] - 2 * m[5] * w[14] - xy6 * w[15];
+            ez += m[4] * w[10] + 10 * m[5] * w[11] + 3 * q * w[12] + 10 * m[7] * w[13] + m[8] * w[14];
+        }
+        // d = v / |v|: dL/dv = (e - d (d . e)) / |v|
+        const double dot = d.x * ex + d.y * ey + d.z * ez;
+        g_mean[0] += (ex - d.x * dot) * d.inv;
+        g_mean[1] += (ey - d.y * dot) * d.inv;
+        g_mean[2] += (ez - d.z * dot) * d.inv;
     }
+#pragma unroll
+    for (int k = 0; k < 48; k++) acc[k] *= (float)BASIS_CONST[k & 15];
     float4 *out = d_sh + (size_t)i * 12;
 #pragma unroll
     for (int v = 0; v < 12; v++) {
@@ -204,12 +265,15 @@ extern "C" int gs_sh_color(gs_ctx *ctx, int32_t N, const uint32_t *words, const 
     if (rc || N == 0 || n_views == 0) return rc;
     GS_REQUIRE(means && colors && clamped, "gs_sh_color: NULL array argument");
     GS_HIP(hipSetDevice(ctx->device));
+    // the degree is a template argument: its tests are a select per term otherwise
+    auto kern = degree == 0 ? sh_color_kernel<0> : degree == 1 ? sh_color_kernel<1> : degree == 2 ? sh_color_kernel<2>
+                                                                                           : sh_color_kernel<3>;
     for (int done = 0; done < n_views;) {
         Cameras cams;
         const int n = take_cameras(&cams, cam_pos, done, n_views);
         { gs_prof_scope prof_(ctx, GS_K_SH_COLOR);
-          hipLaunchKernelGGL(sh_color_kernel, dim3(blocks_of(N)), dim3(256), 0, ctx->stream, N,
-                             reinterpret_cast<const uint4 *>(words), means, degree, cams, colors + 3 * (size_t)N * done,
+          hipLaunchKernelGGL(kern, dim3(blocks_of(N)), dim3(256), 0, ctx->stream, N,
+                             reinterpret_cast<const uint4 *>(words), means, cams, colors + 3 * (size_t)N * done,
                              clamped + 3 * (size_t)N * done); }
         GS_HIP(hipGetLastError());
         done += n;
@@ -227,13 +291,17 @@ extern "C" int gs_sh_color_backward(gs_ctx *ctx, int32_t N, const uint32_t *word
                "gs_sh_color_backward: NULL array argument");
     GS_REQUIRE(((uintptr_t)dL_dsh & 15) == 0, "gs_sh_color_backward: dL_dsh must be 16-byte aligned");
     GS_HIP(hipSetDevice(ctx->device));
+    auto kern = degree == 0   ? sh_color_backward_kernel<0>
+                : degree == 1 ? sh_color_backward_kernel<1>
+                : degree == 2 ? sh_color_backward_kernel<2>
+                              : sh_color_backward_kernel<3>;
     int done = 0;
     do {      // no views: one launch that writes zeros (or adds nothing)
         Cameras cams;
         const int n = take_cameras(&cams, cam_pos, done, n_views);
         { gs_prof_scope prof_(ctx, GS_K_SH_COLOR);
-          hipLaunchKernelGGL(sh_color_backward_kernel, dim3(blocks_of(N)), dim3(256), 0, ctx->stream, N,
-                             reinterpret_cast<const uint4 *>(words), means, degree, cams,
+          hipLaunchKernelGGL(kern, dim3(blocks_of(N)), dim3(256), 0, ctx->stream, N,
+                             reinterpret_cast<const uint4 *>(words), means, cams,
                              clamped + 3 * (size_t)N * done, dL_dcolors + 3 * (size_t)N * done,
                              (accumulate || done > 0) ? 1 : 0, reinterpret_cast<float4 *>(dL_dsh), dL_dmeans); }
         GS_HIP(hipGetLastError());

@@ -34,20 +34,33 @@ __device__ __forceinline__ float gs_half_bits(uint32_t h) {
     return (float)c.f;
 }
 
-// the 48 coefficients [channel][k], as floats
+typedef float gs_float2 __attribute__((ext_vector_type(2)));
+
+// two codes (byte B of w) times the scale whose exponent bits `scale` holds: exact for every scale byte, NaN for 255
+template <int B>
+__device__ __forceinline__ void gs_e2m1_pair(uint32_t w, float scale, float &a, float &b) {
+    const gs_float2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, B);
+    a = v.x;
+    b = v.y;
+}
+
+// The 48 coefficients [channel][k], as floats: 24 conversions by the hardware's own E2M1 instruction.
 __device__ __forceinline__ void gs_sh_decode(const gs_sh_record &r, float (&coef)[48]) {
 #pragma unroll
     for (int ch = 0; ch < 3; ch++) {
-        coef[16 * ch] = gs_half_bits(ch == 0 ? r.w[0] & 0xffffu : ch == 1 ? r.w[0] >> 16 : r.w[1] & 0xffffu);
-        const uint32_t s = gs_sh_scale(r, ch);
-        const bool bad = s == GS_SH_SCALE_NAN;
-#pragma unroll
-        for (int k = 1; k < 16; k++) {
-            const uint32_t c = r.w[2 + 2 * ch + (k - 1) / 8] >> (4 * ((k - 1) & 7));
-            // the code's exponent and mantissa as the top bits of a float: 2^-126 of its value (.5 is a denormal there)
-            const float f = __uint_as_float(((c & 8u) << 28) | ((c & 7u) << 22));
-            coef[16 * ch + k] = bad ? __uint_as_float(0x7fc00000u) : ldexpf(f, (int)s - 1);
-        }
+        float *c = coef + 16 * ch;
+        c[0] = gs_half_bits(ch == 0 ? r.w[0] & 0xffffu : ch == 1 ? r.w[0] >> 16 : r.w[1] & 0xffffu);
+        const float scale = __uint_as_float(gs_sh_scale(r, ch) << 23);
+        const uint32_t lo = r.w[2 + 2 * ch], hi = r.w[3 + 2 * ch];
+        float unused;                       // the last nibble belongs to a scale byte
+        gs_e2m1_pair<0>(lo, scale, c[1], c[2]);
+        gs_e2m1_pair<1>(lo, scale, c[3], c[4]);
+        gs_e2m1_pair<2>(lo, scale, c[5], c[6]);
+        gs_e2m1_pair<3>(lo, scale, c[7], c[8]);
+        gs_e2m1_pair<0>(hi, scale, c[9], c[10]);
+        gs_e2m1_pair<1>(hi, scale, c[11], c[12]);
+        gs_e2m1_pair<2>(hi, scale, c[13], c[14]);
+        gs_e2m1_pair<3>(hi, scale, c[15], unused);
     }
 }
 
@@ -60,11 +73,18 @@ __device__ __forceinline__ uint32_t gs_sh_block_scale(uint32_t amax) {
     return (uint32_t)(e < 0 ? 0 : e > GS_SH_SCALE_MAX ? GS_SH_SCALE_MAX : e);
 }
 
-// E2M1 code of v in a block of scale s (not NaN): to nearest, ties to the even code, 6 at most
-__device__ __forceinline__ uint32_t gs_e2m1_code(float v, uint32_t s) {
-    const float x = fabsf(v) * __uint_as_float((254u - s) << 23);     // exact, or below half the smallest step
-    uint32_t c = (x > 0.25f) + (x >= 0.75f) + (x > 1.25f) + (x >= 1.75f) + (x > 2.5f) + (x >= 3.5f) + (x > 5.0f);
-    return c | ((__float_as_uint(v) >> 28) & 8u);
+// The 15 codes of a channel (c[1..15]) in a block of scale byte s, 255 excepted: to nearest, ties to the even code, 6 scales
+// at most -- what the hardware's conversion does.
+__device__ __forceinline__ void gs_sh_codes(const float *c, uint32_t s, uint32_t &lo, uint32_t &hi) {
+    const float scale = __uint_as_float(s << 23);
+    lo = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, c[1], c[2], scale, 0);
+    lo = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(lo, c[3], c[4], scale, 1);
+    lo = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(lo, c[5], c[6], scale, 2);
+    lo = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(lo, c[7], c[8], scale, 3);
+    hi = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, c[9], c[10], scale, 0);
+    hi = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(hi, c[11], c[12], scale, 1);
+    hi = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(hi, c[13], c[14], scale, 2);
+    hi = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(hi, c[15], 0.0f, scale, 3);
 }
 
 // half-precision bits of a constant term: to nearest even; finite values saturate, infinities and NaN stay

@@ -20,6 +20,44 @@ struct Cameras {
     int n;
 };
 
+// The [N][48] floats that a wave's 64 threads hold leave through LDS: a column per thread on one side, memory order (12
+// stores of 1 KiB of whole lines) on the other.  Threads that store their own 192 bytes write 64 quarter lines per store
+// instead (dequantising 5 M gaussians 205 us against 302).  One wave's LDS operations execute in order and no other wave
+// uses its columns: no barrier.  Pitch 261: both sides are free of bank conflicts.
+// (Loads do not gain: the cache holds the quarter lines until they are asked for, and the LDS costs waves: quantising 5 M
+// 321 us through LDS, 250 with direct loads.)
+constexpr int COLUMN_PITCH = 261;
+typedef float4 Columns[12][COLUMN_PITCH];
+
+// wave-uniform: the wave's first gaussian and how many it has (64, or fewer in the last wave)
+struct Rows {
+    uint32_t first, n;
+};
+__device__ __forceinline__ Rows wave_rows(int N) {
+    const uint32_t first = blockIdx.x * 256u + (threadIdx.x & ~63u);
+    return {first, first >= (uint32_t)N ? 0u : min(64u, (uint32_t)N - first)};
+}
+
+template <bool ADD>
+__device__ __forceinline__ void registers_to_rows(Columns &s, const Rows r, const float (&c)[48], float4 *__restrict__ dst) {
+    const int lane = threadIdx.x & 63, col0 = threadIdx.x & ~63;
+#pragma unroll
+    for (int v = 0; v < 12; v++) s[v][threadIdx.x] = make_float4(c[4 * v], c[4 * v + 1], c[4 * v + 2], c[4 * v + 3]);
+    float4 *p = dst + (size_t)r.first * 12;
+#pragma unroll
+    for (int k = 0; k < 12; k++) {
+        const uint32_t j = k * 64 + lane;                // float4 j of the wave's 768: gaussian j / 12, quarter j % 12
+        if (j < r.n * 12) {
+            float4 f = s[j % 12][col0 + j / 12];
+            if (ADD) {
+                const float4 old = p[j];
+                f.x += old.x; f.y += old.y; f.z += old.z; f.w += old.w;
+            }
+            p[j] = f;
+        }
+    }
+}
+
 __global__ __launch_bounds__(256) void sh_quantize_kernel(int N, const float4 *__restrict__ sh, uint4 *__restrict__ words) {
     const uint32_t i = blockIdx.x * 256u + threadIdx.x;
     if (i >= (uint32_t)N) return;
@@ -37,15 +75,11 @@ __global__ __launch_bounds__(256) void sh_quantize_kernel(int N, const float4 *_
 #pragma unroll
         for (int k = 1; k < 16; k++) amax = max(amax, __float_as_uint(c[16 * ch + k]) & 0x7fffffffu);
         s[ch] = gs_sh_block_scale(amax);
-        uint32_t lo = 0, hi = 0;
-        if (s[ch] != GS_SH_SCALE_NAN) {
-#pragma unroll
-            for (int k = 1; k < 16; k++) {
-                const uint32_t code = gs_e2m1_code(c[16 * ch + k], s[ch]);
-                if (k < 9) lo |= code << (4 * (k - 1)); else hi |= code << (4 * (k - 9));
-            }
-        }
-        r.w[2 + 2 * ch] = lo; r.w[3 + 2 * ch] = hi;
+        uint32_t lo, hi;
+        gs_sh_codes(c + 16 * ch, s[ch], lo, hi);
+        const bool bad = s[ch] == GS_SH_SCALE_NAN;
+        r.w[2 + 2 * ch] = bad ? 0u : lo;
+        r.w[3 + 2 * ch] = bad ? 0u : hi;
     }
     r.w[0] = gs_half_code(c[0]) | gs_half_code(c[16]) << 16;
     r.w[1] = gs_half_code(c[32]) | s[0] << 16 | s[1] << 24;
@@ -56,12 +90,11 @@ __global__ __launch_bounds__(256) void sh_quantize_kernel(int N, const float4 *_
 }
 
 __global__ __launch_bounds__(256) void sh_dequantize_kernel(int N, const uint4 *__restrict__ words, float4 *__restrict__ sh) {
+    __shared__ Columns s_col;
     const uint32_t i = blockIdx.x * 256u + threadIdx.x;
-    if (i >= (uint32_t)N) return;
     float c[48];
-    gs_sh_decode(gs_sh_load(words, i), c);
-#pragma unroll
-    for (int v = 0; v < 12; v++) sh[(size_t)i * 12 + v] = make_float4(c[4 * v], c[4 * v + 1], c[4 * v + 2], c[4 * v + 3]);
+    gs_sh_decode(gs_sh_load(words, min(i, (uint32_t)N - 1)), c);
+    registers_to_rows<false>(s_col, wave_rows(N), c, sh);
 }
 
 // ---- colour.  On the unit sphere the 16 basis functions are constants times these polynomials (x^2 + y^2 + z^2 = 1 turns
@@ -143,8 +176,9 @@ __global__ __launch_bounds__(256) void sh_color_backward_kernel(int N, const uin
                                                                 const float *__restrict__ d_colors, int accumulate,
                                                                 float4 *__restrict__ d_sh, float *__restrict__ d_means) {
     constexpr int NB = (DEGREE + 1) * (DEGREE + 1);
-    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
-    if (i >= (uint32_t)N) return;
+    __shared__ Columns s_col;
+    const uint32_t own = blockIdx.x * 256u + threadIdx.x;
+    const uint32_t i = min(own, (uint32_t)N - 1);      // threads behind the last gaussian repeat it and store nothing
     float coef[48], acc[48];
     gs_sh_decode(gs_sh_load(words, i), coef);
 #pragma unroll
@@ -154,15 +188,31 @@ __global__ __launch_bounds__(256) void sh_color_backward_kernel(int N, const uin
     }
     const double x = means[3 * (size_t)i], y = means[3 * (size_t)i + 1], z = means[3 * (size_t)i + 2];
     double g_mean[3] = {0, 0, 0};
+    // a view's gradients and flags are fetched one view ahead of their use, flags or no flags: three loads whose latency
+    // the view in front of them covers
+    struct Inputs {
+        float g[3];
+        uint8_t clamped[3];
+    };
+    auto fetch = [&](int v) {
+        Inputs in;
+        const size_t o = 3 * ((size_t)v * N + i);
+#pragma unroll
+        for (int ch = 0; ch < 3; ch++) { in.g[ch] = d_colors[o + ch]; in.clamped[ch] = clamped[o + ch]; }
+        return in;
+    };
+    Inputs next = {};
+    if (cams.n > 0) next = fetch(0);
 #pragma unroll 1
     for (int v = 0; v < cams.n; v++) {
+        const Inputs in = next;
+        next = fetch(min(v + 1, cams.n - 1));
         const Direction d = direction(x, y, z, cams.pos[v]);
         const float dx = (float)d.x, dy = (float)d.y, dz = (float)d.z;
         float m[16], w[16], g[3];
         basis_polynomials<DEGREE, float>(dx, dy, dz, m);
-        const size_t o = 3 * ((size_t)v * N + i);
 #pragma unroll
-        for (int ch = 0; ch < 3; ch++) g[ch] = clamped[o + ch] ? 0.0f : d_colors[o + ch];
+        for (int ch = 0; ch < 3; ch++) g[ch] = in.clamped[ch] ? 0.0f : in.g[ch];
 #pragma unroll
         for (int k = 0; k < NB; k++) {
             w[k] = __builtin_fmaf(g[2], coef[32 + k], __builtin_fmaf(g[1], coef[16 + k], g[0] * coef[k]));
@@ -192,16 +242,9 @@ __global__ __launch_bounds__(256) void sh_color_backward_kernel(int N, const uin
     }
 #pragma unroll
     for (int k = 0; k < 48; k++) acc[k] *= (float)BASIS_CONST[k & 15];
-    float4 *out = d_sh + (size_t)i * 12;
-#pragma unroll
-    for (int v = 0; v < 12; v++) {
-        float4 f = make_float4(acc[4 * v], acc[4 * v + 1], acc[4 * v + 2], acc[4 * v + 3]);
-        if (accumulate) {
-            const float4 old = out[v];
-            f.x += old.x; f.y += old.y; f.z += old.z; f.w += old.w;
-        }
-        out[v] = f;
-    }
+    if (accumulate) registers_to_rows<true>(s_col, wave_rows(N), acc, d_sh);
+    else registers_to_rows<false>(s_col, wave_rows(N), acc, d_sh);
+    if (own >= (uint32_t)N) return;
 #pragma unroll
     for (int k = 0; k < 3; k++) {
         const size_t o = 3 * (size_t)i + k;

@@ -12,7 +12,7 @@
 namespace {
 
 // N may be the largest int32
-unsigned blocks_of(int32_t N) { return ((unsigned)N + 255u) / 256u; }
+unsigned blocks_of(int32_t N, unsigned per_block = 256) { return ((unsigned)N + per_block - 1) / per_block; }
 
 constexpr int MAX_COLOR_VIEWS = 32;      // camera positions that one launch takes by value
 struct Cameras {
@@ -58,35 +58,38 @@ __device__ __forceinline__ void registers_to_rows(Columns &s, const Rows r, cons
     }
 }
 
-__global__ __launch_bounds__(256) void sh_quantize_kernel(int N, const float4 *__restrict__ sh, uint4 *__restrict__ words) {
-    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
-    if (i >= (uint32_t)N) return;
-    float c[48];
+// A thread per channel: its 64 bytes in four loads (a thread per gaussian asks for 192 bytes in twelve, more lines in
+// flight than the cache holds: 250 us for 5 M gaussians against XXX).  The three threads of a gaussian, which may sit in
+// different waves, meet in LDS, and the records leave 16 bytes per thread.
+constexpr int QUANT_GAUSSIANS = 64;
+__global__ __launch_bounds__(3 * QUANT_GAUSSIANS) void sh_quantize_kernel(int N, const float4 *__restrict__ sh,
+                                                                          uint4 *__restrict__ words) {
+    __shared__ uint4 s_row[3 * QUANT_GAUSSIANS];      // codes lo, hi; scale; half-precision constant
+    const uint32_t first = blockIdx.x * (uint32_t)QUANT_GAUSSIANS;
+    const uint32_t n = min((uint32_t)QUANT_GAUSSIANS, (uint32_t)N - first);
+    if (threadIdx.x < 3 * n) {
+        const float4 *p = sh + ((size_t)first * 3 + threadIdx.x) * 4;
+        float c[16];
 #pragma unroll
-    for (int v = 0; v < 12; v++) {
-        const float4 f = sh[(size_t)i * 12 + v];
-        c[4 * v] = f.x; c[4 * v + 1] = f.y; c[4 * v + 2] = f.z; c[4 * v + 3] = f.w;
-    }
-    gs_sh_record r;
-    uint32_t s[3];
-#pragma unroll
-    for (int ch = 0; ch < 3; ch++) {
+        for (int v = 0; v < 4; v++) {
+            const float4 f = p[v];
+            c[4 * v] = f.x; c[4 * v + 1] = f.y; c[4 * v + 2] = f.z; c[4 * v + 3] = f.w;
+        }
         uint32_t amax = 0;
 #pragma unroll
-        for (int k = 1; k < 16; k++) amax = max(amax, __float_as_uint(c[16 * ch + k]) & 0x7fffffffu);
-        s[ch] = gs_sh_block_scale(amax);
+        for (int k = 1; k < 16; k++) amax = max(amax, __float_as_uint(c[k]) & 0x7fffffffu);
+        const uint32_t s = gs_sh_block_scale(amax);
+        const bool bad = s == GS_SH_SCALE_NAN;
         uint32_t lo, hi;
-        gs_sh_codes(c + 16 * ch, s[ch], lo, hi);
-        const bool bad = s[ch] == GS_SH_SCALE_NAN;
-        r.w[2 + 2 * ch] = bad ? 0u : lo;
-        r.w[3 + 2 * ch] = bad ? 0u : hi;
+        gs_sh_codes(c, s, lo, hi);
+        s_row[threadIdx.x] = make_uint4(bad ? 0u : lo, bad ? 0u : hi, s, gs_half_code(c[0]));
     }
-    r.w[0] = gs_half_code(c[0]) | gs_half_code(c[16]) << 16;
-    r.w[1] = gs_half_code(c[32]) | s[0] << 16 | s[1] << 24;
-    r.w[3] |= s[2] << 28;
-    r.w[5] |= (s[2] >> 4) << 28;
-    words[2 * (size_t)i] = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
-    words[2 * (size_t)i + 1] = make_uint4(r.w[4], r.w[5], r.w[6], r.w[7]);
+    __syncthreads();
+    if (threadIdx.x >= 2 * n) return;
+    const uint4 r = s_row[3 * (threadIdx.x >> 1)], g = s_row[3 * (threadIdx.x >> 1) + 1], b = s_row[3 * (threadIdx.x >> 1) + 2];
+    words[2 * (size_t)first + threadIdx.x] =
+        threadIdx.x & 1 ? make_uint4(g.x, g.y | (b.z >> 4) << 28, b.x, b.y)
+                        : make_uint4(r.w | g.w << 16, b.w | r.z << 16 | g.z << 24, r.x, r.y | b.z << 28);
 }
 
 __global__ __launch_bounds__(256) void sh_dequantize_kernel(int N, const uint4 *__restrict__ words, float4 *__restrict__ sh) {
@@ -283,7 +286,7 @@ extern "C" int gs_sh_quantize(gs_ctx *ctx, int32_t N, const float *sh, uint32_t 
     GS_REQUIRE(sh && ((uintptr_t)sh & 15) == 0, "gs_sh_quantize: sh must be a 16-byte aligned array");
     GS_HIP(hipSetDevice(ctx->device));
     { gs_prof_scope prof_(ctx, GS_K_SH_PACK);
-      hipLaunchKernelGGL(sh_quantize_kernel, dim3(blocks_of(N)), dim3(256), 0, ctx->stream, N,
+      hipLaunchKernelGGL(sh_quantize_kernel, dim3(blocks_of(N, QUANT_GAUSSIANS)), dim3(3 * QUANT_GAUSSIANS), 0, ctx->stream, N,
                          reinterpret_cast<const float4 *>(sh), reinterpret_cast<uint4 *>(words)); }
     GS_HIP(hipGetLastError());
     return GS_OK;

@@ -114,19 +114,17 @@ SIGNATURES = {
                                     _F, _F, _F, _I32, _I32, _F]),
     "gs_sh_quantize": (ctypes.c_int, [_P, _I32, _P, _P]),
     "gs_sh_dequantize": (ctypes.c_int, [_P, _I32, _P, _P]),
-    "gs_sh_color": (ctypes.c_int, [_P, _I32, _P, _P, _I32, _I32, ctypes.POINTER(ctypes.c_double), _P, _P]),
-    "gs_sh_color_backward": (ctypes.c_int, [_P, _I32, _P, _P, _I32, _I32, ctypes.POINTER(ctypes.c_double), _P, _P, _I32, _P,
-                                            _P]),
+    "gs_sh_color": (ctypes.c_int, [_P, _I32, _P, _P, _I32, _I32, _P, _P, _P]),
+    "gs_sh_color_backward": (ctypes.c_int, [_P, _I32, _P, _P, _I32, _I32, _P, _P, _P, _I32, _P, _P]),
     "gs_ctx_use_packed_sh": (ctypes.c_int, [_P, _I32, _P]),
     "gs_preprocess_batch_records_views": (ctypes.c_int, [_P, _I32, _P, _P, _P, _P, _P, _I64, _I32,
                                                          ctypes.POINTER(GsViewRecords)]),
     "gs_backward_params_batch_scaled": (ctypes.c_int, [_P, _I32, _P, _P, _P, _P, _P, _I32, _I32,
                                                        ctypes.POINTER(GsViewBackward), ctypes.POINTER(_F), _I32, _P, _P, _P,
                                                        _P, _P]),
-    "gs_opacity_dropout": (ctypes.c_int, [_P, _I32, _P, _I32, ctypes.c_double, ctypes.c_uint64, _I32,
-                                          ctypes.POINTER(ctypes.c_uint64), _P]),
-    "gs_opacity_dropout_backward": (ctypes.c_int, [_P, _I32, _P, _I32, ctypes.c_double, ctypes.c_uint64, _I32,
-                                                   ctypes.POINTER(ctypes.c_uint64), _P, _I32, _P]),
+    "gs_opacity_dropout": (ctypes.c_int, [_P, _I32, _P, _I32, ctypes.c_double, ctypes.c_uint64, _I32, _P, _P]),
+    "gs_opacity_dropout_backward": (ctypes.c_int, [_P, _I32, _P, _I32, ctypes.c_double, ctypes.c_uint64, _I32, _P, _P, _I32,
+                                                   _P]),
     "rasterize_tile": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_int, ctypes.c_int,
                                       ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
 }

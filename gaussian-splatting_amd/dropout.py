@@ -20,7 +20,7 @@ from ._lib import check
 
 def _view_ids(views):
     ids = [int(v) for v in views]
-    if any(v < 0 or v >= 2 ** 64 for v in ids):
+    if ids and (min(ids) < 0 or max(ids) >= 2 ** 64):
         raise ValueError("view numbers must be in 0 .. 2^64 - 1")
     return (ctypes.c_uint64 * max(len(ids), 1))(*ids), len(ids)
 

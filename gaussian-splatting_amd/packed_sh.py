@@ -107,13 +107,13 @@ def camera_position(camera_r, camera_t):
 
 
 def _positions(cam_pos):
-    p = np.asarray(cam_pos.detach().cpu() if _is_t(cam_pos) else cam_pos, dtype=np.float64)
+    """([V][3] doubles on the host, V); a copy, so that the array passed in may be read-only or strided."""
+    p = np.array(cam_pos.detach().cpu() if _is_t(cam_pos) else cam_pos, dtype=np.float64, order="C")
     if p.size == 0:
-        p = p.reshape(0, 3)
+        return (ctypes.c_double * 1)(), 0
     if p.ndim not in (1, 2) or p.shape[-1] != 3:
         raise ValueError(f"cam_pos must be [V,3] (or [3] for one camera), got {list(p.shape)}")
-    p = np.ascontiguousarray(p.reshape(-1, 3))
-    return p, p.shape[0], p.ctypes.data_as(ctypes.POINTER(ctypes.c_double))
+    return (ctypes.c_double * p.size).from_buffer(p), p.size // 3
 
 
 def _means(means, packed, c):
@@ -129,7 +129,7 @@ def sh_color(packed, means, cam_pos, degree=3, ctx=None):
     c.sync_stream()
     words = _words(packed, c)
     m = _means(means, packed, c)
-    _held, V, pos = _positions(cam_pos)
+    pos, V = _positions(cam_pos)
     N = len(packed)
     colors = torch.empty((V, N, 3), dtype=torch.float32, device=c.device)
     clamped = torch.empty((V, N, 3), dtype=torch.uint8, device=c.device)
@@ -149,7 +149,7 @@ def sh_color_backward(packed, means, cam_pos, clamped, d_colors, degree=3, ctx=N
     c.sync_stream()
     words = _words(packed, c)
     m = _means(means, packed, c)
-    _held, V, pos = _positions(cam_pos)
+    pos, V = _positions(cam_pos)
     N = len(packed)
     for name, t in (("clamped", clamped), ("d_colors", d_colors)):
         if tuple(t.shape) != (V, N, 3) and not (V == 1 and tuple(t.shape) == (N, 3)):

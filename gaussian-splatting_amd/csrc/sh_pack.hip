@@ -20,6 +20,13 @@ struct Cameras {
     int n;
 };
 
+// Outputs that nothing on the chip reads again before they have left its caches: non-temporal stores (dequantising 5 M
+// gaussians 178 us against 192, gradients 1 view 10 M 426 against 446).
+__device__ __forceinline__ void store_streaming(float4 *p, const float4 f) {
+    typedef float vec4 __attribute__((ext_vector_type(4)));
+    __builtin_nontemporal_store(vec4{f.x, f.y, f.z, f.w}, reinterpret_cast<vec4 *>(p));
+}
+
 // The [N][48] floats that a wave's 64 threads hold leave through LDS: a column per thread on one side, memory order (12
 // stores of 1 KiB of whole lines) on the other.  Threads that store their own 192 bytes write 64 quarter lines per store
 // instead (dequantising 5 M gaussians 205 us against 302).  One wave's LDS operations execute in order and no other wave
@@ -53,14 +60,14 @@ __device__ __forceinline__ void registers_to_rows(Columns &s, const Rows r, cons
                 const float4 old = p[j];
                 f.x += old.x; f.y += old.y; f.z += old.z; f.w += old.w;
             }
-            p[j] = f;
+            store_streaming(p + j, f);
         }
     }
 }
 
-// A thread per channel: its 64 bytes in four loads (a thread per gaussian asks for 192 bytes in twelve, more lines in
-// flight than the cache holds: 250 us for 5 M gaussians against XXX).  The three threads of a gaussian, which may sit in
-// different waves, meet in LDS, and the records leave 16 bytes per thread.
+// A thread per channel: its 64 bytes in four loads.  The three threads of a gaussian, which may sit in different waves, meet
+// in LDS, and the records leave 16 bytes per thread.  1 M gaussians 40 us = 5.6 TB/s, 5 M 205 us (a thread per gaussian,
+// twelve loads 192 bytes apart: 43 and 208; non-temporal loads drop the lines between them: 100 and 487).
 constexpr int QUANT_GAUSSIANS = 64;
 __global__ __launch_bounds__(3 * QUANT_GAUSSIANS) void sh_quantize_kernel(int N, const float4 *__restrict__ sh,
                                                                           uint4 *__restrict__ words) {
@@ -141,7 +148,7 @@ __device__ __forceinline__ Direction direction(double x, double y, double z, con
 
 // In fp64 from the difference of the positions on, as K1 evaluates colours: the flag is the sign of the sum.
 template <int DEGREE>
-__global__ __launch_bounds__(256) void sh_color_kernel(int N, const uint4 *__restrict__ words, const float *__restrict__ means,
+__global__ __launch_bounds__(256, 4) void sh_color_kernel(int N, const uint4 *__restrict__ words, const float *__restrict__ means,
                                                        const Cameras cams, float *__restrict__ colors,
                                                        uint8_t *__restrict__ clamped) {
     constexpr int NB = (DEGREE + 1) * (DEGREE + 1);
@@ -164,7 +171,7 @@ __global__ __launch_bounds__(256) void sh_color_kernel(int N, const uint4 *__res
 #pragma unroll
             for (int k = 0; k < NB; k++) r = __builtin_fma(m[k], (double)coef[16 * ch + k], r);
             const bool c = r < 0;
-            colors[o + ch] = c ? 0.0f : (float)r;
+            __builtin_nontemporal_store(c ? 0.0f : (float)r, colors + o + ch);
             clamped[o + ch] = c;
         }
     }

@@ -146,33 +146,83 @@ __device__ __forceinline__ Direction direction(double x, double y, double z, con
     return d;
 }
 
-// In fp64 from the difference of the positions on, as K1 evaluates colours: the flag is the sign of the sum.
+// The colour as a polynomial a(x, y) + z b(x, y): zz = 1 - xx - yy leaves ten terms of degree 3 in a and six of degree 2 in
+// b, as many as there are coefficients, and Horner's rule needs no monomials: 15 multiply-adds per channel and view.
+struct Polynomial {
+    double a[10], b[6];      // a: 1, x, xx, xxx, y, xy, xxy, yy, xyy, yyy;  b: 1, x, xx, y, xy, yy
+};
 template <int DEGREE>
+__device__ __forceinline__ Polynomial polynomial(const float *coef) {
+    double c[16];
+#pragma unroll
+    for (int k = 0; k < 16; k++) c[k] = k < (DEGREE + 1) * (DEGREE + 1) ? BASIS_CONST[k] * (double)coef[k] : 0.0;
+    Polynomial p{};
+    p.a[0] = 0.5 + c[0];
+    if (DEGREE > 0) { p.a[1] = c[3]; p.a[4] = c[1]; p.b[0] = c[2]; }
+    if (DEGREE > 1) {
+        p.a[0] += 2 * c[6]; p.a[2] = c[8] - 3 * c[6]; p.a[5] = c[4]; p.a[7] = -c[8] - 3 * c[6];
+        p.b[1] = c[7]; p.b[3] = c[5];
+    }
+    if (DEGREE > 2) {
+        p.a[1] += 4 * c[13]; p.a[3] = c[15] - 5 * c[13]; p.a[4] += 4 * c[11]; p.a[6] = 3 * c[9] - 5 * c[11];
+        p.a[8] = -3 * c[15] - 5 * c[13]; p.a[9] = -c[9] - 5 * c[11];
+        p.b[0] += 2 * c[12]; p.b[2] = c[14] - 5 * c[12]; p.b[4] = c[10]; p.b[5] = -c[14] - 5 * c[12];
+    }
+    return p;
+}
+template <int DEGREE>
+__device__ __forceinline__ double evaluate(const Polynomial &p, double x, double y, double z) {
+    auto fma = [](double a, double b, double c) { return __builtin_fma(a, b, c); };
+    if (DEGREE == 0) return p.a[0];
+    if (DEGREE == 1) return fma(x, p.a[1], fma(y, p.a[4], fma(z, p.b[0], p.a[0])));
+    if (DEGREE == 2) {
+        const double a = fma(y, fma(y, p.a[7], fma(x, p.a[5], p.a[4])), fma(x, fma(x, p.a[2], p.a[1]), p.a[0]));
+        return fma(z, fma(y, p.b[3], fma(x, p.b[1], p.b[0])), a);
+    }
+    const double a0 = fma(x, fma(x, fma(x, p.a[3], p.a[2]), p.a[1]), p.a[0]), a1 = fma(x, fma(x, p.a[6], p.a[5]), p.a[4]);
+    const double a = fma(y, fma(y, fma(y, p.a[9], fma(x, p.a[8], p.a[7])), a1), a0);
+    const double b = fma(y, fma(y, p.b[5], fma(x, p.b[4], p.b[3])), fma(x, fma(x, p.b[2], p.b[1]), p.b[0]));
+    return fma(z, b, a);
+}
+
+// In fp64 from the difference of the positions on, as K1 evaluates colours: the flag is the sign of the sum.
+// SEVERAL views are bound by the fp64 arithmetic of the view loop, and turning the coefficients into a Polynomial in front of
+// it pays: 1 M gaussians x 8 views 36 us = 4.6 TB/s (42 without), 3 M x 4 views 64 (67).  A single view does not earn that
+// back and stays at the memory's rate without: 10 M gaussians 103 us = 5.7 TB/s (117 with).
+template <int DEGREE, bool SEVERAL>
 __global__ __launch_bounds__(256, 4) void sh_color_kernel(int N, const uint4 *__restrict__ words, const float *__restrict__ means,
-                                                       const Cameras cams, float *__restrict__ colors,
-                                                       uint8_t *__restrict__ clamped) {
+                                                          const Cameras cams, float *__restrict__ colors,
+                                                          uint8_t *__restrict__ clamped) {
     constexpr int NB = (DEGREE + 1) * (DEGREE + 1);
     const uint32_t i = blockIdx.x * 256u + threadIdx.x;
     if (i >= (uint32_t)N) return;
     float coef[48];
     gs_sh_decode(gs_sh_load(words, i), coef);
     const double x = means[3 * (size_t)i], y = means[3 * (size_t)i + 1], z = means[3 * (size_t)i + 2];
+    const size_t o = 3 * (size_t)i;
+    auto store = [&](size_t at, double r) {
+        const bool c = r < 0;
+        __builtin_nontemporal_store(c ? 0.0f : (float)r, colors + at);
+        clamped[at] = c;
+    };
+    if (SEVERAL) {
+        const Polynomial p[3] = {polynomial<DEGREE>(coef), polynomial<DEGREE>(coef + 16), polynomial<DEGREE>(coef + 32)};
 #pragma unroll 1
-    for (int v = 0; v < cams.n; v++) {
-        const Direction d = direction(x, y, z, cams.pos[v]);
+        for (int v = 0; v < cams.n; v++) {
+            const Direction d = direction(x, y, z, cams.pos[v]);
+#pragma unroll
+            for (int ch = 0; ch < 3; ch++) store(3 * (size_t)N * v + o + ch, evaluate<DEGREE>(p[ch], d.x, d.y, d.z));
+        }
+    } else {
+        const Direction d = direction(x, y, z, cams.pos[0]);
         double m[16];
         basis_polynomials<DEGREE, double>(d.x, d.y, d.z, m);
-#pragma unroll
-        for (int k = 0; k < NB; k++) m[k] *= BASIS_CONST[k];
-        const size_t o = 3 * ((size_t)v * N + i);
 #pragma unroll
         for (int ch = 0; ch < 3; ch++) {
             double r = 0.5;
 #pragma unroll
-            for (int k = 0; k < NB; k++) r = __builtin_fma(m[k], (double)coef[16 * ch + k], r);
-            const bool c = r < 0;
-            __builtin_nontemporal_store(c ? 0.0f : (float)r, colors + o + ch);
-            clamped[o + ch] = c;
+            for (int k = 0; k < NB; k++) r = __builtin_fma(m[k] * BASIS_CONST[k], (double)coef[16 * ch + k], r);
+            store(o + ch, r);
         }
     }
 }
@@ -319,13 +369,14 @@ extern "C" int gs_sh_color(gs_ctx *ctx, int32_t N, const uint32_t *words, const 
     GS_REQUIRE(means && colors && clamped, "gs_sh_color: NULL array argument");
     GS_HIP(hipSetDevice(ctx->device));
     // the degree is a template argument: its tests are a select per term otherwise
-    auto kern = degree == 0 ? sh_color_kernel<0> : degree == 1 ? sh_color_kernel<1> : degree == 2 ? sh_color_kernel<2>
-                                                                                           : sh_color_kernel<3>;
+    constexpr decltype(&sh_color_kernel<0, false>) kernels[2][4] = {
+        {sh_color_kernel<0, false>, sh_color_kernel<1, false>, sh_color_kernel<2, false>, sh_color_kernel<3, false>},
+        {sh_color_kernel<0, true>, sh_color_kernel<1, true>, sh_color_kernel<2, true>, sh_color_kernel<3, true>}};
     for (int done = 0; done < n_views;) {
         Cameras cams;
         const int n = take_cameras(&cams, cam_pos, done, n_views);
         { gs_prof_scope prof_(ctx, GS_K_SH_COLOR);
-          hipLaunchKernelGGL(kern, dim3(blocks_of(N)), dim3(256), 0, ctx->stream, N,
+          hipLaunchKernelGGL(kernels[n > 1][degree], dim3(blocks_of(N)), dim3(256), 0, ctx->stream, N,
                              reinterpret_cast<const uint4 *>(words), means, cams, colors + 3 * (size_t)N * done,
                              clamped + 3 * (size_t)N * done); }
         GS_HIP(hipGetLastError());
@@ -344,16 +395,14 @@ extern "C" int gs_sh_color_backward(gs_ctx *ctx, int32_t N, const uint32_t *word
                "gs_sh_color_backward: NULL array argument");
     GS_REQUIRE(((uintptr_t)dL_dsh & 15) == 0, "gs_sh_color_backward: dL_dsh must be 16-byte aligned");
     GS_HIP(hipSetDevice(ctx->device));
-    auto kern = degree == 0   ? sh_color_backward_kernel<0>
-                : degree == 1 ? sh_color_backward_kernel<1>
-                : degree == 2 ? sh_color_backward_kernel<2>
-                              : sh_color_backward_kernel<3>;
+    constexpr decltype(&sh_color_backward_kernel<0>) kernels[4] = {sh_color_backward_kernel<0>, sh_color_backward_kernel<1>,
+                                                                   sh_color_backward_kernel<2>, sh_color_backward_kernel<3>};
     int done = 0;
     do {      // no views: one launch that writes zeros (or adds nothing)
         Cameras cams;
         const int n = take_cameras(&cams, cam_pos, done, n_views);
         { gs_prof_scope prof_(ctx, GS_K_SH_COLOR);
-          hipLaunchKernelGGL(kern, dim3(blocks_of(N)), dim3(256), 0, ctx->stream, N,
+          hipLaunchKernelGGL(kernels[degree], dim3(blocks_of(N)), dim3(256), 0, ctx->stream, N,
                              reinterpret_cast<const uint4 *>(words), means, cams,
                              clamped + 3 * (size_t)N * done, dL_dcolors + 3 * (size_t)N * done,
                              (accumulate || done > 0) ? 1 : 0, reinterpret_cast<float4 *>(dL_dsh), dL_dmeans); }

@@ -382,3 +382,108 @@ def test_on_another_stream(gpu_ctx):
         packed = gs.quantize_sh(buf, ctx=gpu_ctx)
     torch.cuda.current_stream(d).wait_stream(side)
     np.testing.assert_array_equal(packed.numpy()[:200], want)
+
+
+def test_offsets_past_32_bits(gpu_ctx):
+    """More than 4 GiB of coefficients, colours and opacities: the last rows are those of a call on them alone."""
+    import torch
+    import gsplat_amd as gs
+    d, n, tail = gpu_ctx.device, 23_000_001, 777
+    sh = torch.rand((n, 3, 16), device=d) - 0.5                       # 4.4 GB
+    packed = gs.quantize_sh(sh, ctx=gpu_ctx)
+    last = gs.quantize_sh(sh[-tail:], ctx=gpu_ctx)
+    assert torch.equal(packed.words[-tail:], last.words)
+    del sh
+    dense = packed.dequantize(gpu_ctx)
+    assert torch.equal(dense[-tail:], last.dequantize(gpu_ctx))
+    del dense
+    means = torch.rand((n, 3), device=d) + torch.tensor([0., 0., 5.], device=d)
+    V = 17
+    cams = np.random.default_rng(0).uniform(-1, 1, (V, 3))
+    col, cl = gs.sh_color(packed, means, cams, ctx=gpu_ctx)           # 4.7 GB
+    c1, f1 = gs.sh_color(last, means[-tail:], cams, ctx=gpu_ctx)
+    assert torch.equal(col[:, -tail:], c1) and torch.equal(cl[:, -tail:], f1)
+    d_sh, d_means = gs.sh_color_backward(packed, means, cams, cl, col, ctx=gpu_ctx)
+    e_sh, e_means = gs.sh_color_backward(last, means[-tail:], cams, f1, c1, ctx=gpu_ctx)
+    assert torch.equal(d_sh[-tail:], e_sh) and torch.equal(d_means[-tail:], e_means)
+    del col, cl, d_sh
+    x, views = torch.ones(n, device=d), list(range(100, 148))
+    out = gs.dropout_opacity(x, .5, 9, views, ctx=gpu_ctx)             # 4.4 GB
+    for i in (0, n // 2, n - 2, n - 1):
+        keep = [packed_ref.philox((i, 0, v >> 2, 0), (9, 0))[v & 3] >= 2 ** 31 for v in views]
+        assert (out[:, i] != 0).tolist() == keep
+    back = gs.dropout_opacity_backward(out, x, .5, 9, views, ctx=gpu_ctx)
+    assert float(back[-1]) == 4.0 * sum(keep) and float(back[0]) == 2.0 * float(out[:, 0].sum())
+
+
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_misaligned_inputs(gpu_ctx, offset):
+    """Gradients, flags, positions and opacities that start at any float or byte."""
+    import torch
+    import gsplat_amd as gs
+    d, n, V = gpu_ctx.device, 301, 3
+
+    def shifted(t):
+        flat = torch.zeros(t.numel() + offset, dtype=t.dtype, device=d)
+        flat[offset:] = t.reshape(-1)
+        return flat[offset:].view(t.shape)
+    gen = torch.Generator().manual_seed(offset)
+    packed = gs.quantize_sh(torch.randn((n, 3, 16), generator=gen).to(d), ctx=gpu_ctx)
+    means = (torch.randn((n, 3), generator=gen) + torch.tensor([0., 0., 9.])).to(d)
+    cams = np.random.default_rng(1).uniform(-1, 1, (2 * V, 3))[::2]                  # strided on the host
+    col, cl = gs.sh_color(packed, means, cams, ctx=gpu_ctx)
+    g = torch.randn((V, n, 3), generator=gen).to(d)
+    want = gs.sh_color_backward(packed, means, cams, cl, g, ctx=gpu_ctx)
+    got = gs.sh_color_backward(packed, shifted(means), cams, shifted(cl), shifted(g), ctx=gpu_ctx)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(gs.sh_color(packed, shifted(means), cams, ctx=gpu_ctx)[0], col)
+    strided = g.permute(2, 1, 0).contiguous().permute(2, 1, 0)
+    got = gs.sh_color_backward(packed, means, cams, cl, strided, ctx=gpu_ctx)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    part = gs.PackedSH(packed.words[1:])                                              # records from the second on
+    assert torch.equal(gs.sh_color(part, means[1:], cams, ctx=gpu_ctx)[0], col[:, 1:])
+    x, gx = torch.randn(n, generator=gen).to(d), torch.randn((V, n), generator=gen).to(d)
+    assert torch.equal(gs.dropout_opacity(shifted(x), .3, 2, range(V), True, ctx=gpu_ctx),
+                       gs.dropout_opacity(x, .3, 2, range(V), True, ctx=gpu_ctx))
+    assert torch.equal(gs.dropout_opacity_backward(shifted(gx), shifted(x), .3, 2, range(V), True, ctx=gpu_ctx),
+                       gs.dropout_opacity_backward(gx, x, .3, 2, range(V), True, ctx=gpu_ctx))
+
+
+def test_numpy_in_numpy_out(gpu_ctx):
+    import gsplat_amd as gs
+    words, means = packed_ref.quantize(_sh(20)), _means(20).astype(np.float64)
+    cam = np.array([.1, .2, .3])                                                       # one camera, [3]
+    cam.setflags(write=False)
+    col, cl = gs.sh_color(gs.PackedSH(words), means, cam, ctx=gpu_ctx)                 # records on the host
+    assert col.dtype == np.float64 and cl.dtype == np.uint8 and col.shape == (1, 20, 3)
+    want = packed_ref.color(packed_ref.dequantize(words), means.astype(np.float32), cam, 3)
+    np.testing.assert_allclose(col, np.maximum(want, 0), rtol=2 * U, atol=1e-12)
+    d_sh, d_means = gs.sh_color_backward(gs.PackedSH(words), means, cam, cl[0], np.ones((20, 3)), ctx=gpu_ctx)
+    assert d_sh.shape == (20, 3, 16) and d_means.dtype == np.float64
+    g = gs.dropout_opacity_backward(np.ones(20), np.full(20, .5), .25, 1, [6], ctx=gpu_ctx)
+    np.testing.assert_allclose(g, np.where(packed_ref.keep_mask(20, .25, 1, [6])[0], 4 / 3, 0), rtol=4 * U)
+
+
+def test_nothing_outside_the_outputs_is_written(gpu_ctx):
+    """Guard words around every output buffer that the caller owns."""
+    import torch
+    import gsplat_amd as gs
+    d, n, V = gpu_ctx.device, 131, 2
+    packed = gs.quantize_sh(torch.from_numpy(_sh(n)).to(d), ctx=gpu_ctx)
+    means = torch.from_numpy(_means(n)).to(d)
+    cams = np.zeros((V, 3))
+
+    def guarded(shape):
+        k = int(np.prod(shape))
+        buf = torch.full((k + 128,), 7.5, device=d)
+        return buf, buf[64:64 + k].view(shape)
+    b1, d_sh = guarded((n, 3, 16))
+    b2, d_means = guarded((n, 3))
+    b3, d_op = guarded((n,))
+    col, cl = gs.sh_color(packed, means, cams, ctx=gpu_ctx)
+    gs.sh_color_backward(packed, means, cams, cl, col, ctx=gpu_ctx, out=(d_sh, d_means))
+    gs.dropout_opacity_backward(torch.ones((V, n), device=d), torch.ones(n, device=d), .1, 0, [0, 1], ctx=gpu_ctx, out=d_op)
+    for b in (b1, b2, b3):
+        assert (b[:64] == 7.5).all() and (b[-64:] == 7.5).all()
+    want = gs.sh_color_backward(packed, means, cams, cl, col, ctx=gpu_ctx)
+    assert torch.equal(d_sh, want[0]) and torch.equal(d_means, want[1])

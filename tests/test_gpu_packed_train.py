@@ -292,3 +292,19 @@ def test_changed_coefficients_are_packed_again(gpu_ctx):
     b, _ = pipe.forward(view)
     c, _ = pipe.forward(view, pre=pipe.preprocess_batch([view])[0])
     assert not torch.equal(a, b) and torch.equal(b, c)
+
+
+def test_densifier_does_not_count_left_out_views(gpu_ctx):
+    import torch
+    import gsplat_amd as gs
+    cam, g, rs = _scene(400)
+    g.opacity = np.abs(g.opacity)
+    pipe = gs.SplatPipeline(g, rs, ctx=gpu_ctx)
+    den = gs.Densifier(pipe)
+    views, targets = _views(gs, cam, 4), _targets(gpu_ctx, rs, 4)
+    radii = [st["radii"] for st in pipe.preprocess_batch(views)]
+    gs.train_step(pipe, views, targets, gs.FlatGrads(pipe.N, gpu_ctx.device), concurrent_views=2, states_hook=den.accumulate,
+                  dropout=gs.OpacityDropout(.5, 3, first_view=40))
+    keep = torch.from_numpy(packed_ref.keep_mask(pipe.N, .5, 3, range(40, 44))).to(gpu_ctx.device)
+    want = sum(((r > 0) & k).float() for r, k in zip(radii, keep))
+    assert torch.equal(den.denom, want) and 0 < float(want.sum()) < sum(int((r > 0).sum()) for r in radii)

@@ -3,8 +3,9 @@
 // gradients (sh_backpass + kernel sh_grads, backward_pass.py:70-97, setup_gpu.py:256-303).  The reference keeps its
 // coefficients in full precision only.
 //
-// All four kernels are bound by HBM: per gaussian 192 + 32 bytes (conversions), 44 + 15 V (colour of V views),
-// 44 + 15 V + 204 (its gradients).  One thread per gaussian.
+// What they have to move per gaussian: 192 + 32 bytes (conversions), 44 + 15 V (colour of V views), 44 + 15 V + 204 (its
+// gradients).  All are bound by HBM, at the 5.0-5.2 TB/s a large copy reaches or above, but for colours and gradients of many
+// views, which the arithmetic of the view loop bounds (figures at the kernels).
 #include "common.h"
 #include "precam.h"
 #include "sh_pack.h"
@@ -31,8 +32,7 @@ __device__ __forceinline__ void store_streaming(float4 *p, const float4 f) {
 // stores of 1 KiB of whole lines) on the other.  Threads that store their own 192 bytes write 64 quarter lines per store
 // instead (dequantising 5 M gaussians 205 us against 302).  One wave's LDS operations execute in order and no other wave
 // uses its columns: no barrier.  Pitch 261: both sides are free of bank conflicts.
-// (Loads do not gain: the cache holds the quarter lines until they are asked for, and the LDS costs waves: quantising 5 M
-// 321 us through LDS, 250 with direct loads.)
+// Half the pitch in two rounds, for twice the waves, is slower (208 us against 178).
 constexpr int COLUMN_PITCH = 261;
 typedef float4 Columns[12][COLUMN_PITCH];
 
@@ -99,6 +99,7 @@ __global__ __launch_bounds__(3 * QUANT_GAUSSIANS) void sh_quantize_kernel(int N,
                         : make_uint4(r.w | g.w << 16, b.w | r.z << 16 | g.z << 24, r.x, r.y | b.z << 28);
 }
 
+// 1 M gaussians 35 us, 5 M 178 us = 6.3 TB/s.
 __global__ __launch_bounds__(256) void sh_dequantize_kernel(int N, const uint4 *__restrict__ words, float4 *__restrict__ sh) {
     __shared__ Columns s_col;
     const uint32_t i = blockIdx.x * 256u + threadIdx.x;
@@ -229,6 +230,9 @@ __global__ __launch_bounds__(256, 4) void sh_color_kernel(int N, const uint4 *__
 
 // fp32 behind the fp64 direction, as in K8: products and sums of a few dozen terms.  The constants of the basis are taken
 // out of the view loop: they are multiplied into the coefficients in front of it and into the sums behind it.
+// 10 M gaussians x 1 view 426 us = 6.2 TB/s, 3 M x 4 views 175 us = 5.3, 1 M x 8 views 84 us = 4.4: some 215 vector
+// instructions per view and wave (93 of them the products of w and acc) bound the last.  The coefficients and sums of a
+// gaussian hold 96 registers: three waves per SIMD; four (half the LDS per wave, spilled registers) take 156 us.
 template <int DEGREE>
 __global__ __launch_bounds__(256) void sh_color_backward_kernel(int N, const uint4 *__restrict__ words,
                                                                 const float *__restrict__ means, const Cameras cams,

@@ -8,7 +8,8 @@ the backward pass evaluates it again, and every rank and device gets the same on
     train_step(pipe, views, targets, grads, dropout=OpacityDropout(p, seed, first_view=step * len(views)))
 
 Arrays may be NumPy (results come back as NumPy, float64) or torch tensors (results stay on the device).  Calls run on
-torch's current stream of the context's device and do not synchronise."""
+torch's current stream of the context's device and do not synchronise.  Seed and view numbers are read when the call is
+made: a captured graph replays the masks it was captured with."""
 import ctypes
 
 import numpy as np

@@ -86,6 +86,8 @@ def _aligned(t):
 def quantize_sh(sh, ctx=None):
     """SH coefficients [N,3,16] -> PackedSH (gs_sh_quantize).  Per (gaussian, channel) the 15 coefficients behind the
     constant term share a power-of-two scale and are rounded to 4 bits (E2M1); the constant term to half precision."""
+    if isinstance(sh, PackedSH):
+        raise TypeError("the coefficients are packed already")
     c = _ctx(ctx)
     c.sync_stream()
     shape = tuple(sh.shape)

@@ -88,6 +88,10 @@ def test_refused_before_a_launch():
         gs.PackedSH(np.zeros((4, 8)), ctx=c)
     packed = _packed(5)
     assert packed.shape == (5, 3, 16) and len(packed[1:3]) == 2 and packed.nbytes == 160
+    with pytest.raises(TypeError, match="packed already"):
+        gs.quantize_sh(packed, ctx=c)
+    with pytest.raises(IndexError, match="slice"):
+        packed[2]
     with pytest.raises(TypeError, match="quantize_sh"):
         gs.sh_color(torch.zeros(5, 3, 16), torch.zeros(5, 3), np.zeros((1, 3)), ctx=c)
     with pytest.raises(ValueError, match="means"):

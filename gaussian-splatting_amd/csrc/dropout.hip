@@ -8,29 +8,33 @@
 //
 // They have to move 4 + 4 V bytes per gaussian forward, 8 + 4 V backward, and to evaluate the generator once per gaussian
 // and block of four view numbers -- once per view for the views a rank of a multi-rank job renders, whose numbers lie apart.
-// That evaluation, some 70 instructions, bounds them: 10 M gaussians x 4 views of different blocks 60 us = 3.3 TB/s, the
-// gradient 63 us; 1 M x 8 views 18.5 us.  A thread takes four gaussians (one: 86 and 151 us, two: 69 and 93).
+// That evaluation, some 70 instructions, bounds them: 10 M gaussians x 4 views of different blocks 57 us = 3.5 TB/s, the
+// gradient 60 us; 1 M x 8 views 17.8 us.
 #include "common.h"
 #include <math.h>
 #include <string.h>
 
 namespace {
 
-// N may be the largest int32
-unsigned blocks_of(int32_t N) { return ((unsigned)N + 1023u) / 1024u; }      // 256 threads of PER_THREAD gaussians
-
 // The views of a launch, grouped by the evaluation of the generator they share: up to four views of one block s >> 2, each
-// with another word.  Built on the host; a number that is there twice starts a group of its own.
+// with another word.  Built on the host; a number that is there twice starts a group of its own.  A group is one 16-byte
+// scalar load in the kernels.
 constexpr int MAX_DROP_GROUPS = 32, MAX_DROP_VIEWS = 64;
+constexpr uint32_t NO_VIEW = 255;
+struct alignas(16) ViewGroup {
+    uint64_t block;
+    uint32_t views;           // byte k: the launch's view that takes word k, or NO_VIEW
+    uint32_t unused;
+    __host__ __device__ uint32_t view(int k) const { return (views >> (8 * k)) & 255u; }
+};
 struct ViewGroups {
-    uint64_t block[MAX_DROP_GROUPS];
-    int8_t view[MAX_DROP_GROUPS][4];      // the launch's view that takes word k, -1: none
+    ViewGroup g[MAX_DROP_GROUPS];
     int n;
 };
 
 // Nine of the generator's ten rounds; a view's word needs one of the last round's two products.
 // The 64-bit products are what it spends its time on (17 that depend on the gaussian, at a quarter of the rate of other
-// instructions), the exclusive ors come second: three operands each (two by two: 76 us instead of 60).
+// instructions), the exclusive ors come second: three operands each (two by two: 76 us instead of 57).
 constexpr uint32_t M0 = 0xD2511F53u, M1 = 0xCD9E8D57u, W0 = 0x9E3779B9u, W1 = 0xBB67AE85u;
 __device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
 
@@ -60,102 +64,138 @@ __device__ __forceinline__ void last_round(const State &s, uint64_t seed, uint32
 
 __device__ __forceinline__ float activated(float x, int is_logit) { return is_logit ? 1.0f / (1.0f + expf(-x)) : x; }
 
-// four neighbouring gaussians per thread: rows of N floats start at any multiple of 4 bytes
-constexpr int PER_THREAD = 4;
-typedef float row4 __attribute__((ext_vector_type(4), aligned(4)));
+// PER neighbouring gaussians per thread, loaded and stored together; rows of N floats start at any multiple of 4 bytes.
+// `all` is uniform in a block: the last block of a launch goes element by element.
+template <int PER>
+struct Row {
+    typedef float vec __attribute__((ext_vector_type(PER), aligned(4)));
+    float v[PER];
+    __device__ __forceinline__ void load(const float *p, bool all, uint32_t n) {
+        if (all) {
+            const vec t = *reinterpret_cast<const vec *>(p);
+#pragma unroll
+            for (int e = 0; e < PER; e++) v[e] = t[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < PER; e++) v[e] = e < (int)n ? p[e] : 0.0f;
+        }
+    }
+    __device__ __forceinline__ void store(float *p, bool all, uint32_t n) const {
+        if (all) {
+            vec t;
+#pragma unroll
+            for (int e = 0; e < PER; e++) t[e] = v[e];
+            *reinterpret_cast<vec *>(p) = t;
+        } else {
+#pragma unroll
+            for (int e = 0; e < PER; e++)
+                if (e < (int)n) p[e] = v[e];
+        }
+    }
+};
+template <>
+struct Row<1> {
+    float v[1];
+    __device__ __forceinline__ void load(const float *p, bool, uint32_t) { v[0] = *p; }
+    __device__ __forceinline__ void store(float *p, bool, uint32_t) const { *p = v[0]; }
+};
 
+template <int PER>
 __global__ __launch_bounds__(256) void opacity_dropout_kernel(int N, const float *__restrict__ opacity, int is_logit,
                                                               uint32_t limit, float scale, uint64_t seed, const ViewGroups groups,
                                                               float *__restrict__ out) {
-    const uint32_t i = (blockIdx.x * 256u + threadIdx.x) * PER_THREAD;
+    const uint32_t i = (blockIdx.x * 256u + threadIdx.x) * PER;
     if (i >= (uint32_t)N) return;
-    const uint32_t n = min((uint32_t)PER_THREAD, (uint32_t)N - i);
-    row4 x = {0, 0, 0, 0};
-    if (n == PER_THREAD) x = *reinterpret_cast<const row4 *>(opacity + i);
-    else
-        for (uint32_t e = 0; e < n; e++) x[e] = opacity[i + e];
+    const bool all = (blockIdx.x + 1) * (256u * PER) <= (uint32_t)N;
+    const uint32_t n = min((uint32_t)PER, (uint32_t)N - i);
+    Row<PER> x;
+    x.load(opacity + i, all, n);
 #pragma unroll
-    for (int e = 0; e < PER_THREAD; e++) x[e] = activated(x[e], is_logit) * scale;
+    for (int e = 0; e < PER; e++) x.v[e] = activated(x.v[e], is_logit) * scale;
 #pragma unroll 1
     for (int g = 0; g < groups.n; g++) {
-        State s[PER_THREAD];
+        const ViewGroup group = groups.g[g];
+        State s[PER];
 #pragma unroll
-        for (int e = 0; e < PER_THREAD; e++) s[e] = nine_rounds(i + e, groups.block[g], seed);
+        for (int e = 0; e < PER; e++) s[e] = nine_rounds(i + e, group.block, seed);
 #pragma unroll
         for (int pair = 0; pair < 2; pair++) {
-            if (groups.view[g][2 * pair] < 0 && groups.view[g][2 * pair + 1] < 0) continue;
-            uint32_t w[2][PER_THREAD];
+            if (group.view(2 * pair) == NO_VIEW && group.view(2 * pair + 1) == NO_VIEW) continue;
+            uint32_t w[2][PER];
 #pragma unroll
-            for (int e = 0; e < PER_THREAD; e++) {
+            for (int e = 0; e < PER; e++) {
                 if (pair == 0) last_round<0>(s[e], seed, w[0][e], w[1][e]);
                 else last_round<1>(s[e], seed, w[0][e], w[1][e]);
             }
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                const int v = groups.view[g][2 * pair + k];
-                if (v < 0) continue;
-                row4 y;
+                const uint32_t v = group.view(2 * pair + k);
+                if (v == NO_VIEW) continue;
+                Row<PER> y;
 #pragma unroll
-                for (int e = 0; e < PER_THREAD; e++) y[e] = w[k][e] >= limit ? x[e] : 0.0f;
-                float *p = out + ((size_t)v * N + i);
-                if (n == PER_THREAD) *reinterpret_cast<row4 *>(p) = y;
-                else
-                    for (uint32_t e = 0; e < n; e++) p[e] = y[e];
+                for (int e = 0; e < PER; e++) y.v[e] = w[k][e] >= limit ? x.v[e] : 0.0f;
+                y.store(out + ((size_t)v * N + i), all, n);
             }
         }
     }
 }
 
+template <int PER>
 __global__ __launch_bounds__(256) void opacity_dropout_backward_kernel(int N, const float *__restrict__ opacity, int is_logit,
                                                                        uint32_t limit, float scale, uint64_t seed,
                                                                        const ViewGroups groups, const float *__restrict__ d_out,
                                                                        int accumulate, float *__restrict__ d_opacity) {
-    const uint32_t i = (blockIdx.x * 256u + threadIdx.x) * PER_THREAD;
+    const uint32_t i = (blockIdx.x * 256u + threadIdx.x) * PER;
     if (i >= (uint32_t)N) return;
-    const uint32_t n = min((uint32_t)PER_THREAD, (uint32_t)N - i);
-    row4 sum = {0, 0, 0, 0};
+    const bool all = (blockIdx.x + 1) * (256u * PER) <= (uint32_t)N;
+    const uint32_t n = min((uint32_t)PER, (uint32_t)N - i);
+    Row<PER> sum = {};
 #pragma unroll 1
     for (int g = 0; g < groups.n; g++) {
-        row4 d[4];
+        const ViewGroup group = groups.g[g];
+        Row<PER> d[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {                   // in flight while the generator runs
-            const int v = groups.view[g][k];
-            d[k] = row4{0, 0, 0, 0};
-            if (v < 0) continue;
-            const float *p = d_out + ((size_t)v * N + i);
-            if (n == PER_THREAD) d[k] = *reinterpret_cast<const row4 *>(p);
-            else
-                for (uint32_t e = 0; e < n; e++) d[k][e] = p[e];
+            const uint32_t v = group.view(k);
+            d[k] = {};
+            if (v != NO_VIEW) d[k].load(d_out + ((size_t)v * N + i), all, n);
         }
-        State s[PER_THREAD];
+        State s[PER];
 #pragma unroll
-        for (int e = 0; e < PER_THREAD; e++) s[e] = nine_rounds(i + e, groups.block[g], seed);
+        for (int e = 0; e < PER; e++) s[e] = nine_rounds(i + e, group.block, seed);
 #pragma unroll
         for (int pair = 0; pair < 2; pair++) {
-            if (groups.view[g][2 * pair] < 0 && groups.view[g][2 * pair + 1] < 0) continue;
+            if (group.view(2 * pair) == NO_VIEW && group.view(2 * pair + 1) == NO_VIEW) continue;
 #pragma unroll
-            for (int e = 0; e < PER_THREAD; e++) {
+            for (int e = 0; e < PER; e++) {
                 uint32_t w0, w1;
                 if (pair == 0) last_round<0>(s[e], seed, w0, w1);
                 else last_round<1>(s[e], seed, w0, w1);
                 // selected: a NaN of a dropped gaussian stays out
-                sum[e] += w0 >= limit ? d[2 * pair][e] : 0.0f;
-                sum[e] += w1 >= limit ? d[2 * pair + 1][e] : 0.0f;
+                sum.v[e] += w0 >= limit ? d[2 * pair].v[e] : 0.0f;
+                sum.v[e] += w1 >= limit ? d[2 * pair + 1].v[e] : 0.0f;
             }
         }
     }
+    Row<PER> r;
+    if (is_logit) {
+        r.load(opacity + i, all, n);
 #pragma unroll
-    for (int e = 0; e < PER_THREAD; e++) {
-        if (e >= (int)n) break;
-        float f = sum[e];
-        if (is_logit) {
-            const float o = activated(opacity[i + e], 1);
-            f *= o * (1.0f - o);
+        for (int e = 0; e < PER; e++) {
+            const float o = activated(r.v[e], 1);
+            sum.v[e] *= o * (1.0f - o);
         }
-        f *= scale;
-        d_opacity[i + e] = accumulate ? d_opacity[i + e] + f : f;
     }
+    if (accumulate) r.load(d_opacity + i, all, n);
+#pragma unroll
+    for (int e = 0; e < PER; e++) r.v[e] = accumulate ? r.v[e] + sum.v[e] * scale : sum.v[e] * scale;
+    r.store(d_opacity + i, all, n);
 }
+
+// Gaussians per thread: four share a view's scalar work and store 16 bytes at once, but leave small scenes with few waves.
+// us forward / backward with one and with four: 10 k x 8 views 7.3 / 7.3 and 9.2 / 9.6, 300 k x 8 9.7 / 9.3 and 11.7 / 11.5,
+// 1 M x 8 18.2 / 17.8 and 17.8 / 17.2, 10 M x 4 63 / 69 and 57 / 60.
+inline int per_thread(int32_t N) { return N >= (1 << 19) ? 4 : 1; }
 
 int check_dropout(const char *who, gs_ctx *ctx, int32_t N, double p, int32_t n_views, const uint64_t *view_ids, uint32_t *limit,
                   float *scale) {
@@ -174,17 +214,20 @@ int take_views(ViewGroups *out, const uint64_t *ids, int first, int n_views) {
     int v = 0;
     for (; first + v < n_views && v < MAX_DROP_VIEWS; v++) {
         const uint64_t id = ids[first + v];
-        int g = out->n - 1;
-        if (g < 0 || out->block[g] != id >> 2 || out->view[g][id & 3] >= 0) {
+        const int k = (int)(id & 3);
+        ViewGroup *g = out->n ? &out->g[out->n - 1] : nullptr;
+        if (!g || g->block != id >> 2 || g->view(k) != NO_VIEW) {
             if (out->n == MAX_DROP_GROUPS) break;
-            g = out->n++;
-            out->block[g] = id >> 2;
-            for (int k = 0; k < 4; k++) out->view[g][k] = -1;
+            g = &out->g[out->n++];
+            *g = {id >> 2, 0xffffffffu, 0};
         }
-        out->view[g][id & 3] = (int8_t)v;
+        g->views = (g->views & ~(255u << (8 * k))) | (uint32_t)v << (8 * k);
     }
     return v;
 }
+
+// blocks of 256 threads; N may be the largest int32
+unsigned blocks_of(int32_t N, int per) { return ((unsigned)N + 256u * per - 1) / (256u * per); }
 
 }  // namespace
 
@@ -196,11 +239,12 @@ extern "C" int gs_opacity_dropout(gs_ctx *ctx, int32_t N, const float *opacity, 
     if (rc || N == 0 || n_views == 0) return rc;
     GS_REQUIRE(opacity && out, "gs_opacity_dropout: NULL array argument");
     GS_HIP(hipSetDevice(ctx->device));
+    const int per = per_thread(N);
     for (int done = 0; done < n_views;) {
         ViewGroups groups;
         const int n = take_views(&groups, view_ids, done, n_views);
         { gs_prof_scope prof_(ctx, GS_K_DROPOUT);
-          hipLaunchKernelGGL(opacity_dropout_kernel, dim3(blocks_of(N)), dim3(256), 0, ctx->stream, N, opacity,
+          hipLaunchKernelGGL(per == 4 ? opacity_dropout_kernel<4> : opacity_dropout_kernel<1>, dim3(blocks_of(N, per)), dim3(256), 0, ctx->stream, N, opacity,
                              opacity_is_logit, limit, scale, seed, groups, out + (size_t)N * done); }
         GS_HIP(hipGetLastError());
         done += n;
@@ -217,12 +261,13 @@ extern "C" int gs_opacity_dropout_backward(gs_ctx *ctx, int32_t N, const float *
     if (rc || N == 0) return rc;
     GS_REQUIRE(opacity && dL_dopacity && (n_views == 0 || dL_dout), "gs_opacity_dropout_backward: NULL array argument");
     GS_HIP(hipSetDevice(ctx->device));
+    const int per = per_thread(N);
     int done = 0;
     do {      // no views: one launch that writes zeros (or adds nothing)
         ViewGroups groups;
         const int n = take_views(&groups, view_ids, done, n_views);
         { gs_prof_scope prof_(ctx, GS_K_DROPOUT);
-          hipLaunchKernelGGL(opacity_dropout_backward_kernel, dim3(blocks_of(N)), dim3(256), 0, ctx->stream, N, opacity,
+          hipLaunchKernelGGL(per == 4 ? opacity_dropout_backward_kernel<4> : opacity_dropout_backward_kernel<1>, dim3(blocks_of(N, per)), dim3(256), 0, ctx->stream, N, opacity,
                              opacity_is_logit, limit, scale, seed, groups, dL_dout + (size_t)N * done,
                              (accumulate || done > 0) ? 1 : 0, dL_dopacity); }
         GS_HIP(hipGetLastError());

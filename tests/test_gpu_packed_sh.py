@@ -297,6 +297,31 @@ def test_dropout(gpu_ctx, n, views, p, is_logit):
     np.testing.assert_allclose(twice.cpu().numpy(), 2 * got.cpu().numpy(), rtol=2 * U, atol=(len(views) + 2) * U * np.abs(s).sum(axis=0).max() / (1 - p))
 
 
+@pytest.mark.parametrize("n", [(1 << 19) - 1, 1 << 19, (1 << 19) + 1, (1 << 19) + 1022])
+def test_dropout_with_four_gaussians_per_thread(gpu_ctx, n):
+    """Around the size from which a thread takes four, whole and ragged last blocks: the same masks and sums as on parts."""
+    import torch
+    import gsplat_amd as gs
+    d, views = gpu_ctx.device, [3, 2, 9, 9, 40]
+    x = torch.randn(n, generator=torch.Generator().manual_seed(n)).to(d)
+    out = gs.dropout_opacity(x, .4, 11, views, is_logit=True, ctx=gpu_ctx)
+    small = gs.dropout_opacity(x[:1000], .4, 11, views, is_logit=True, ctx=gpu_ctx)
+    assert torch.equal(out[:, :1000], small)
+    for i in (n - 1, n - 2, n - 1023, n // 2):
+        keep = [packed_ref.philox((i, 0, v >> 2, 0), (11, 0))[v & 3] >= int(np.floor(.4 * 2 ** 32 + .5)) for v in views]
+        assert (out[:, i] != 0).tolist() == keep
+    kept = out[out != 0]
+    assert abs(kept.numel() / out.numel() - .6) < 6 * np.sqrt(.24 / (4 * n))             # four different views
+    g = torch.randn((5, n), generator=torch.Generator().manual_seed(1)).to(d)
+    got = gs.dropout_opacity_backward(g, x, .4, 11, views, is_logit=True, ctx=gpu_ctx)
+    s = torch.sigmoid(x.double())
+    want = (torch.where(out != 0, g, torch.zeros_like(g)).double().sum(dim=0) / .6) * s * (1 - s)
+    tol = g.double().abs().sum(dim=0) / .6 * (11 * U * s * (1 - s) + 6 * U * s)
+    assert ((got.double() - want).abs() <= tol).all()
+    again = gs.dropout_opacity_backward(g, x, .4, 11, views, is_logit=True, ctx=gpu_ctx, out=got.clone(), accumulate=True)
+    assert ((again.double() - 2 * got.double()).abs() <= 2 * U * got.double().abs() + tol).all()
+
+
 def test_dropout_edges(gpu_ctx):
     import torch
     import gsplat_amd as gs

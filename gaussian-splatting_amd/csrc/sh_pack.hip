@@ -31,10 +31,13 @@ __device__ __forceinline__ void store_streaming(float4 *p, const float4 f) {
 // The [N][48] floats that a wave's 64 threads hold leave through LDS: a column per thread on one side, memory order (12
 // stores of 1 KiB of whole lines) on the other.  Threads that store their own 192 bytes write 64 quarter lines per store
 // instead (dequantising 5 M gaussians 205 us against 302).  One wave's LDS operations execute in order and no other wave
-// uses its columns: no barrier.  Pitch 261: both sides are free of bank conflicts.
-// Half the pitch in two rounds, for twice the waves, is slower (208 us against 178).
-constexpr int COLUMN_PITCH = 261;
-typedef float4 Columns[12][COLUMN_PITCH];
+// uses its columns: no barrier.  The odd pitch keeps both sides free of bank conflicts.
+// ROUNDS 2: 32 threads at a time, half the LDS, for a kernel that its waves gain by; where LDS does not limit them it costs
+// (dequantising 5 M 208 us against 178).
+template <int ROUNDS>
+struct Columns {
+    float4 q[12][256 / ROUNDS + 5];
+};
 
 // wave-uniform: the wave's first gaussian and how many it has (64, or fewer in the last wave)
 struct Rows {
@@ -45,22 +48,30 @@ __device__ __forceinline__ Rows wave_rows(int N) {
     return {first, first >= (uint32_t)N ? 0u : min(64u, (uint32_t)N - first)};
 }
 
-template <bool ADD>
-__device__ __forceinline__ void registers_to_rows(Columns &s, const Rows r, const float (&c)[48], float4 *__restrict__ dst) {
-    const int lane = threadIdx.x & 63, col0 = threadIdx.x & ~63;
-#pragma unroll
-    for (int v = 0; v < 12; v++) s[v][threadIdx.x] = make_float4(c[4 * v], c[4 * v + 1], c[4 * v + 2], c[4 * v + 3]);
+template <bool ADD, int ROUNDS>
+__device__ __forceinline__ void registers_to_rows(Columns<ROUNDS> &s, const Rows r, const float (&c)[48], float4 *__restrict__ dst) {
+    constexpr int COLS = 64 / ROUNDS;                    // the wave's columns
+    const int lane = threadIdx.x & 63, col0 = (threadIdx.x >> 6) * COLS;
     float4 *p = dst + (size_t)r.first * 12;
 #pragma unroll
-    for (int k = 0; k < 12; k++) {
-        const uint32_t j = k * 64 + lane;                // float4 j of the wave's 768: gaussian j / 12, quarter j % 12
-        if (j < r.n * 12) {
-            float4 f = s[j % 12][col0 + j / 12];
-            if (ADD) {
-                const float4 old = p[j];
-                f.x += old.x; f.y += old.y; f.z += old.z; f.w += old.w;
+    for (int round = 0; round < ROUNDS; round++) {
+        if (ROUNDS == 1 || lane / COLS == round) {
+#pragma unroll
+            for (int v = 0; v < 12; v++)
+                s.q[v][col0 + lane % COLS] = make_float4(c[4 * v], c[4 * v + 1], c[4 * v + 2], c[4 * v + 3]);
+        }
+#pragma unroll
+        for (int k = 0; k < 12 / ROUNDS; k++) {
+            const uint32_t j = k * 64 + lane;            // float4 j of the round: gaussian j / 12, quarter j % 12
+            const uint32_t at = round * COLS * 12 + j;
+            if (at < r.n * 12) {
+                float4 f = s.q[j % 12][col0 + j / 12];
+                if (ADD) {
+                    const float4 old = p[at];
+                    f.x += old.x; f.y += old.y; f.z += old.z; f.w += old.w;
+                }
+                store_streaming(p + at, f);
             }
-            store_streaming(p + j, f);
         }
     }
 }
@@ -101,7 +112,7 @@ __global__ __launch_bounds__(3 * QUANT_GAUSSIANS) void sh_quantize_kernel(int N,
 
 // 1 M gaussians 35 us, 5 M 178 us = 6.3 TB/s.
 __global__ __launch_bounds__(256) void sh_dequantize_kernel(int N, const uint4 *__restrict__ words, float4 *__restrict__ sh) {
-    __shared__ Columns s_col;
+    __shared__ Columns<1> s_col;
     const uint32_t i = blockIdx.x * 256u + threadIdx.x;
     float c[48];
     gs_sh_decode(gs_sh_load(words, min(i, (uint32_t)N - 1)), c);
@@ -229,27 +240,25 @@ __global__ __launch_bounds__(256, 4) void sh_color_kernel(int N, const uint4 *__
 }
 
 // fp32 behind the fp64 direction, as in K8: products and sums of a few dozen terms.  The constants of the basis are taken
-// out of the view loop: they are multiplied into the coefficients in front of it and into the sums behind it.
-// 10 M gaussians x 1 view 426 us = 6.2 TB/s, 3 M x 4 views 175 us = 5.3, 1 M x 8 views 84 us = 4.4: some 215 vector
-// instructions per view and wave (93 of them the products of w and acc) bound the last.  The coefficients and sums of a
-// gaussian hold 96 registers: three waves per SIMD; four (half the LDS per wave, spilled registers) take 156 us.
-template <int DEGREE>
-__global__ __launch_bounds__(256) void sh_color_backward_kernel(int N, const uint4 *__restrict__ words,
-                                                                const float *__restrict__ means, const Cameras cams,
-                                                                const uint8_t *__restrict__ clamped,
-                                                                const float *__restrict__ d_colors, int accumulate,
-                                                                float4 *__restrict__ d_sh, float *__restrict__ d_means) {
+// out of the sums: they are multiplied in behind the view loop.
+// Few views are bound by the rows that are written: the coefficients are decoded once (10 M gaussians x 1 view 427 us = 6.2
+// TB/s).  SEVERAL views are bound by the loop's loads and its 200 vector instructions, and gain more by a fourth wave per SIMD
+// than they lose by decoding the record in every view (45 registers less) and storing in two rounds: 1 M x 8 views 77 us
+// against 85, 3 M x 4 168 against 176; 10 M x 1 466 against 427, 1 M x 2 the same.
+template <int DEGREE, bool SEVERAL>
+__global__ __launch_bounds__(256, SEVERAL ? 4 : 1) void sh_color_backward_kernel(
+    int N, const uint4 *__restrict__ words, const float *__restrict__ means, const Cameras cams,
+    const uint8_t *__restrict__ clamped, const float *__restrict__ d_colors, int accumulate, float4 *__restrict__ d_sh,
+    float *__restrict__ d_means) {
     constexpr int NB = (DEGREE + 1) * (DEGREE + 1);
-    __shared__ Columns s_col;
+    __shared__ Columns<SEVERAL ? 2 : 1> s_col;
     const uint32_t own = blockIdx.x * 256u + threadIdx.x;
     const uint32_t i = min(own, (uint32_t)N - 1);      // threads behind the last gaussian repeat it and store nothing
     float coef[48], acc[48];
-    gs_sh_decode(gs_sh_load(words, i), coef);
+    gs_sh_record record = gs_sh_load(words, i);
+    if (!SEVERAL) gs_sh_decode(record, coef);
 #pragma unroll
-    for (int k = 0; k < 48; k++) {
-        coef[k] *= (float)BASIS_CONST[k & 15];
-        acc[k] = 0.0f;
-    }
+    for (int k = 0; k < 48; k++) acc[k] = 0.0f;
     const double x = means[3 * (size_t)i], y = means[3 * (size_t)i + 1], z = means[3 * (size_t)i + 2];
     double g_mean[3] = {0, 0, 0};
     // a view's gradients and flags are fetched one view ahead of their use, flags or no flags: three loads whose latency
@@ -277,9 +286,14 @@ __global__ __launch_bounds__(256) void sh_color_backward_kernel(int N, const uin
         basis_polynomials<DEGREE, float>(dx, dy, dz, m);
 #pragma unroll
         for (int ch = 0; ch < 3; ch++) g[ch] = in.clamped[ch] ? 0.0f : in.g[ch];
+        if (SEVERAL) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) asm volatile("" : "+v"(record.w[k]));      // decoded here, not in front of the loop
+            gs_sh_decode(record, coef);
+        }
 #pragma unroll
         for (int k = 0; k < NB; k++) {
-            w[k] = __builtin_fmaf(g[2], coef[32 + k], __builtin_fmaf(g[1], coef[16 + k], g[0] * coef[k]));
+            w[k] = (float)BASIS_CONST[k] * __builtin_fmaf(g[2], coef[32 + k], __builtin_fmaf(g[1], coef[16 + k], g[0] * coef[k]));
 #pragma unroll
             for (int ch = 0; ch < 3; ch++) acc[16 * ch + k] = __builtin_fmaf(g[ch], m[k], acc[16 * ch + k]);
         }
@@ -399,14 +413,17 @@ extern "C" int gs_sh_color_backward(gs_ctx *ctx, int32_t N, const uint32_t *word
                "gs_sh_color_backward: NULL array argument");
     GS_REQUIRE(((uintptr_t)dL_dsh & 15) == 0, "gs_sh_color_backward: dL_dsh must be 16-byte aligned");
     GS_HIP(hipSetDevice(ctx->device));
-    constexpr decltype(&sh_color_backward_kernel<0>) kernels[4] = {sh_color_backward_kernel<0>, sh_color_backward_kernel<1>,
-                                                                   sh_color_backward_kernel<2>, sh_color_backward_kernel<3>};
+    constexpr decltype(&sh_color_backward_kernel<0, false>) kernels[2][4] = {
+        {sh_color_backward_kernel<0, false>, sh_color_backward_kernel<1, false>, sh_color_backward_kernel<2, false>,
+         sh_color_backward_kernel<3, false>},
+        {sh_color_backward_kernel<0, true>, sh_color_backward_kernel<1, true>, sh_color_backward_kernel<2, true>,
+         sh_color_backward_kernel<3, true>}};
     int done = 0;
     do {      // no views: one launch that writes zeros (or adds nothing)
         Cameras cams;
         const int n = take_cameras(&cams, cam_pos, done, n_views);
         { gs_prof_scope prof_(ctx, GS_K_SH_COLOR);
-          hipLaunchKernelGGL(kernels[degree], dim3(blocks_of(N)), dim3(256), 0, ctx->stream, N,
+          hipLaunchKernelGGL(kernels[n > 2][degree], dim3(blocks_of(N)), dim3(256), 0, ctx->stream, N,
                              reinterpret_cast<const uint4 *>(words), means, cams,
                              clamped + 3 * (size_t)N * done, dL_dcolors + 3 * (size_t)N * done,
                              (accumulate || done > 0) ? 1 : 0, reinterpret_cast<float4 *>(dL_dsh), dL_dmeans); }

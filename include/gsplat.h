@@ -433,8 +433,9 @@ int gs_sh_dequantize(gs_ctx *ctx, int32_t N, const uint32_t *words, float *sh);
  * forward_pass.py:168-215) of EVERY gaussian (no culling).  cam_pos_host[n_views][3]: HOST doubles, camera_r^T @ camera_t
  * as forward_pass.py:47 forms them.  colors[n_views][N][3] = max(0, .5 + sum_k Y_k(d) c_k) with d the unit vector from
  * the camera position to the mean, clamped[n_views][N][3] = 1 where the sum was negative; coefficients above `degree` do
- * not take part.  Evaluated in fp64: where gs_preprocess does not cull the gaussian, colour and flag are its results on the
- * dequantised coefficients, up to the order of the fp64 sums. */
+ * not take part; a gaussian at the camera's own position gets NaN (degree > 0).  Evaluated in fp64: where gs_preprocess
+ * does not cull the gaussian, colour and flag are its results on the dequantised coefficients, up to the order of the fp64
+ * sums. */
 int gs_sh_color(gs_ctx *ctx, int32_t N, const uint32_t *words, const float *means, int32_t degree, int32_t n_views,
                 const double *cam_pos_host, float *colors, uint8_t *clamped);
 /* Its gradients, summed over the views (sh_backpass + kernel sh_grads, backward_pass.py:70-97, setup_gpu.py:256-303;

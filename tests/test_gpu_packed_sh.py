@@ -512,3 +512,39 @@ def test_nothing_outside_the_outputs_is_written(gpu_ctx):
         assert (b[:64] == 7.5).all() and (b[-64:] == 7.5).all()
     want = gs.sh_color_backward(packed, means, cams, cl, col, ctx=gpu_ctx)
     assert torch.equal(d_sh, want[0]) and torch.equal(d_means, want[1])
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float64"])
+def test_other_float_types_are_taken_as_their_float32_values(gpu_ctx, dtype):
+    import torch
+    import gsplat_amd as gs
+    d, t = gpu_ctx.device, getattr(torch, dtype)
+    sh, means = torch.from_numpy(_sh(70)).to(d).to(t), torch.from_numpy(_means(70)).to(d).to(t)
+    packed = gs.quantize_sh(sh, ctx=gpu_ctx)
+    np.testing.assert_array_equal(packed.numpy(), packed_ref.quantize(sh.float().cpu().numpy()))
+    cam = np.array([[.3, .2, .1]])
+    col, cl = gs.sh_color(packed, means, cam, ctx=gpu_ctx)
+    assert torch.equal(col, gs.sh_color(packed, means.float(), cam, ctx=gpu_ctx)[0])
+    g = torch.randn((1, 70, 3), generator=torch.Generator().manual_seed(0)).to(d).to(t)
+    a, b = (gs.sh_color_backward(packed, means.to(k), cam, cl.bool() if k is t else cl, g.to(k), ctx=gpu_ctx)
+            for k in (t, torch.float32))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    x = torch.randn(70, generator=torch.Generator().manual_seed(1)).to(d).to(t)
+    assert torch.equal(gs.dropout_opacity(x, .2, 1, [5], True, ctx=gpu_ctx), gs.dropout_opacity(x.float(), .2, 1, [5], True, ctx=gpu_ctx))
+
+
+def test_color_at_the_camera_and_far_away(gpu_ctx):
+    """A gaussian at the camera has no direction; one 1e18 away has."""
+    import torch
+    import gsplat_amd as gs
+    d = gpu_ctx.device
+    packed = gs.quantize_sh(torch.from_numpy(_sh(3)).to(d), ctx=gpu_ctx)
+    means = torch.tensor([[1., 2., 3.], [1e18, -2e18, 1e17], [1., 2., 3.0001]], device=d)
+    cam = np.array([[1., 2., 3.]])
+    col, cl = gs.sh_color(packed, means, cam, ctx=gpu_ctx)
+    assert torch.isnan(col[0, 0]).all() and (cl[0, 0] == 0).all()
+    want = packed_ref.color(packed_ref.dequantize(packed.numpy()[1:]), means.cpu().numpy()[1:], cam, 3)
+    np.testing.assert_allclose(col[0, 1:].cpu().numpy(), np.maximum(want[0], 0), rtol=2 * U, atol=1e-12)
+    _, d_means = gs.sh_color_backward(packed, means, cam, cl, torch.ones_like(col), ctx=gpu_ctx)
+    assert torch.isnan(d_means[0]).all() and torch.isfinite(d_means[1:]).all() and float(d_means[1].abs().max()) < 1e-16
+    assert torch.isfinite(gs.sh_color(packed, means, cam, degree=0, ctx=gpu_ctx)[0]).all()

@@ -308,3 +308,26 @@ def test_densifier_does_not_count_left_out_views(gpu_ctx):
     keep = torch.from_numpy(packed_ref.keep_mask(pipe.N, .5, 3, range(40, 44))).to(gpu_ctx.device)
     want = sum(((r > 0) & k).float() for r, k in zip(radii, keep))
     assert torch.equal(den.denom, want) and 0 < float(want.sum()) < sum(int((r > 0).sum()) for r in radii)
+
+
+@pytest.mark.parametrize("lanes", [1, 4])
+def test_step_in_which_every_gaussian_is_left_out(gpu_ctx, lanes):
+    """Empty lists: the background, no gradient, a finite loss."""
+    import torch
+    import gsplat_amd as gs
+    cam, g, rs = _scene(200, 96, 64)
+    assert not packed_ref.keep_mask(200, .9999999, 1, range(4)).any()
+    for cull in (True, False):
+        pipe = gs.SplatPipeline(g, rs, ctx=gpu_ctx, cull_tiles=cull, sh_format="mxfp4", background=(.2, .3, .4))
+        views, targets = _views(gs, cam, 4), _targets(gpu_ctx, rs, 4)
+        drop = gs.OpacityDropout(.9999999, 1)
+        grads = gs.FlatGrads(pipe.N, gpu_ctx.device)
+        grads.flat.fill_(3.0)
+        loss, _ = gs.train_step(pipe, views, targets, grads, concurrent_views=lanes, dropout=drop)
+        bg = torch.tensor([.2, .3, .4], device=gpu_ctx.device)
+        want = sum(((bg - t) ** 2).mean() for t in targets)
+        assert abs(float(loss) - float(want)) <= 1e-5 * float(want)
+        for part in (grads.means, grads.log_scales, grads.quats, grads.opacity, grads.sh):
+            assert (part == 0).all()
+        image, _ = pipe.forward(views[0], pre=pipe.preprocess_batch(views[:1], dropout=drop)[0])
+        assert torch.equal(image, bg.expand_as(image))

@@ -296,7 +296,7 @@ struct PreBatch {
 #else
 #define GS_K1_OCC
 #endif
-template <bool RECORDS, bool FAST, bool PACKED>
+template <bool RECORDS, bool FAST, bool PACKED, bool VIEW_OPACITIES>
 __global__ __launch_bounds__(256) GS_K1_OCC void preprocess_batch_kernel(int N, const float *__restrict__ means,
                                                                const float *__restrict__ log_scales,
                                                                const float *__restrict__ quats,
@@ -311,6 +311,8 @@ __global__ __launch_bounds__(256) GS_K1_OCC void preprocess_batch_kernel(int N, 
     // quarter lines: 0.190 against 0.191 ms per 8 views -- the loads are not what the kernel waits for)
     load_params<PACKED>(i, means, log_scales, quats, sh, x, y, z, q, ls, coef);
     const float opac0 = RECORDS ? opacities[i] : 0.0f;
+    // (VIEW_OPACITIES: opacities of its own per view, opacity_stride apart.  A template argument: what a record holds of the
+    // opacity is formed once for all views otherwise, 235 against 258 us per 8 views)
     // M and Sigma once per gaussian: the host has checked that the views share scale_mod and the scale switch
     double M[9], Sg[9];
     gaussian_cov(b.cam[0].scale_mod, b.cam[0].diag_scale, q[0], q[1], q[2], q[3], ls, M, Sg);
@@ -328,8 +330,7 @@ __global__ __launch_bounds__(256) GS_K1_OCC void preprocess_batch_kernel(int N, 
             reinterpret_cast<int4 *>(w.tiles_touched)[i] = make_int4(o.rect[0], o.rect[1], o.rect[2], o.rect[3]);
 #pragma unroll
             for (int k = 0; k < 3; k++) w.clamped[3 * i + k] = o.cl[k];
-            // (opacity_stride 0: one opacity for every view)
-            const float opac = opacity_stride && v ? opacities[v * opacity_stride + i] : opac0;
+            const float opac = VIEW_OPACITIES && v ? opacities[v * opacity_stride + i] : opac0;
             float4 geo, con, rgb;
             gs_make_record(o.cx, o.cy, opac, o.con[0], o.con[1], o.con[2], o.col[0], o.col[1], o.col[2], geo, con, rgb);
             // The wave's 64 records go through wave-private LDS ([quarter][lane], pitch 68 float4: conflict-free both
@@ -369,10 +370,12 @@ bool pre_fast(const PreBatch &b) {
     return true;
 }
 
-template <bool RECORDS>
+template <bool RECORDS, bool VIEW_OPACITIES>
 auto batch_kernel(const PreBatch &b, bool packed) {
-    return pre_fast(b) ? (packed ? preprocess_batch_kernel<RECORDS, true, true> : preprocess_batch_kernel<RECORDS, true, false>)
-                       : (packed ? preprocess_batch_kernel<RECORDS, false, true> : preprocess_batch_kernel<RECORDS, false, false>);
+    return pre_fast(b) ? (packed ? preprocess_batch_kernel<RECORDS, true, true, VIEW_OPACITIES>
+                                 : preprocess_batch_kernel<RECORDS, true, false, VIEW_OPACITIES>)
+                       : (packed ? preprocess_batch_kernel<RECORDS, false, true, VIEW_OPACITIES>
+                                 : preprocess_batch_kernel<RECORDS, false, false, VIEW_OPACITIES>);
 }
 
 }  // namespace
@@ -473,7 +476,7 @@ extern "C" int gs_preprocess_batch(gs_ctx *ctx, int32_t N, const float *means, c
         }
         done += b.n_views;
         { gs_prof_scope prof_(ctx, GS_K_PREPROCESS);
-          auto kern = batch_kernel<false>(b, packed);
+          auto kern = batch_kernel<false, false>(b, packed);
           hipLaunchKernelGGL(kern, dim3(gs_div_up(N, 256)), dim3(256), 0, ctx->stream, N, means, log_scales, quats, coefs,
                              (const float *)nullptr, (size_t)0, b); }
         GS_HIP(hipGetLastError());
@@ -529,7 +532,7 @@ extern "C" int gs_preprocess_batch_records_views(gs_ctx *ctx, int32_t N, const f
         }
         done += b.n_views;
         { gs_prof_scope prof_(ctx, GS_K_PREPROCESS);
-          auto kern = batch_kernel<true>(b, packed);
+          auto kern = opacity_stride ? batch_kernel<true, true>(b, packed) : batch_kernel<true, false>(b, packed);
           hipLaunchKernelGGL(kern, dim3(gs_div_up(N, 256)), dim3(256), 0, ctx->stream, N, means, log_scales, quats, coefs,
                              view_opacities, (size_t)opacity_stride, b); }
         GS_HIP(hipGetLastError());

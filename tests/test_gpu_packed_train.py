@@ -139,6 +139,13 @@ def test_records_of_another_scene_are_refused(gpu_ctx):
     finally:
         assert lib.gs_ctx_use_packed_sh(h, 0, None) == 0
     pipe.forward(view)
+    null, ptr = ctypes.c_void_p(0), ctypes.c_void_p(pipe.sh.data_ptr())
+    check = import_module("gaussian-splatting_amd._lib").check
+    with pytest.raises(gs.GsError, match="no packed records"):                       # neither coefficients nor records
+        check(lib.gs_preprocess_batch_records(h, 300, ptr, ptr, ptr, null, ptr, 1,
+                                              (import_module("gaussian-splatting_amd._lib").GsViewRecords * 1)()), "K1")
+    with pytest.raises(gs.GsError, match="no packed records"):
+        check(lib.gs_backward_params_batch(h, 300, ptr, ptr, ptr, null, ptr, 0, 0, None, 0, ptr, ptr, ptr, ptr, ptr), "K8")
     with pytest.raises(gs.GsError, match="opacity_stride"):
         import_module("gaussian-splatting_amd._lib").check(lib.gs_preprocess_batch_records_views(h, 300, *([ctypes.c_void_p(pipe.sh.data_ptr())] * 5), 299, 1,
                                                             (import_module("gaussian-splatting_amd._lib").GsViewRecords * 1)()), "views")

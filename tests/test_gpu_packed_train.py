@@ -318,8 +318,11 @@ def test_densifier_does_not_count_left_out_views(gpu_ctx):
 
 
 @pytest.mark.parametrize("lanes", [1, 4])
-def test_step_in_which_every_gaussian_is_left_out(gpu_ctx, lanes):
-    """Empty lists: the background, no gradient, a finite loss."""
+@pytest.mark.parametrize("ordered", [False, True])
+def test_step_in_which_every_gaussian_is_left_out(gpu_ctx, det_ctx, lanes, ordered):
+    """Empty lists, and exact lists whose entries do nothing, with both reductions of the blend backward: the background, no
+    gradient, a finite loss."""
+    gpu_ctx = det_ctx if ordered else gpu_ctx
     import torch
     import gsplat_amd as gs
     cam, g, rs = _scene(200, 96, 64)

@@ -38,7 +38,7 @@ def _stale(target, deps):
 
 def build(force=False, verbose=False):
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
-    headers.append(os.path.join(HERE, "..", "include", "gsplat.h"))
+    headers += [os.path.join(HERE, "..", "include", "gsplat.h"), os.path.abspath(__file__)]      # flags count as a source
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
     objs, procs = [], []

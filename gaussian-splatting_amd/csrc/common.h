@@ -138,6 +138,15 @@ int gs_sh_source(gs_ctx *ctx, const char *who, int32_t N, const float *sh, const
 
 static inline int gs_div_up(int a, int b) { return (a + b - 1) / b; }
 
+// Between the lanes' LDS writes and other lanes' reads of them, and between those reads and the next writes, where only the
+// lanes of one wave exchange.  The hardware executes one wave's LDS operations in order; this keeps the compiler, which
+// orders only what one thread's own addresses make it, from moving them across each other.  No instruction is emitted.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // ---- per-gaussian blend records (blend.hip packs them; the culled binning reads them too) ----
 // one 64-byte record per gaussian, so that staging an entry touches ONE cache line:
 //   [0] geo = cx, cy, opacity, tau     tau = log2(1/255 / opacity) - margin

@@ -30,8 +30,8 @@ __device__ __forceinline__ void store_streaming(float4 *p, const float4 f) {
 
 // The [N][48] floats that a wave's 64 threads hold leave through LDS: a column per thread on one side, memory order (12
 // stores of 1 KiB of whole lines) on the other.  Threads that store their own 192 bytes write 64 quarter lines per store
-// instead (dequantising 5 M gaussians 205 us against 302).  One wave's LDS operations execute in order and no other wave
-// uses its columns: no barrier.  The odd pitch keeps both sides free of bank conflicts.
+// instead (dequantising 5 M gaussians 205 us against 302).  No other wave uses its columns: a fence of the wave on either side
+// of the reads, no barrier.  The odd pitch keeps both sides free of bank conflicts.
 // ROUNDS 2: 32 threads at a time, half the LDS, for a kernel that its waves gain by; where LDS does not limit them it costs
 // (dequantising 5 M 208 us against 178).
 template <int ROUNDS>
@@ -55,11 +55,13 @@ __device__ __forceinline__ void registers_to_rows(Columns<ROUNDS> &s, const Rows
     float4 *p = dst + (size_t)r.first * 12;
 #pragma unroll
     for (int round = 0; round < ROUNDS; round++) {
+        wave_lds_fence();      // the previous round's columns have been read
         if (ROUNDS == 1 || lane / COLS == round) {
 #pragma unroll
             for (int v = 0; v < 12; v++)
                 s.q[v][col0 + lane % COLS] = make_float4(c[4 * v], c[4 * v + 1], c[4 * v + 2], c[4 * v + 3]);
         }
+        wave_lds_fence();
 #pragma unroll
         for (int k = 0; k < 12 / ROUNDS; k++) {
             const uint32_t j = k * 64 + lane;            // float4 j of the round: gaussian j / 12, quarter j % 12

@@ -345,7 +345,7 @@ __global__ __launch_bounds__(256, GS_K8_WAVES) void param_bwd_kernel(
 #endif
     // The SH gradients of a full wave (64 x 192 B, contiguous) leave through the wave's columns of s_sh4, whose
     // coefficients are no longer needed: twelve stores of 1 KiB of whole lines instead of twelve stores of 64 quarter
-    // lines 192 B apart (one wave's LDS operations execute in order: no barrier).
+    // lines 192 B apart (a fence of the wave in front of the reads of other threads' columns, no barrier).
     const int lane = threadIdx.x & 63;
     const bool full_wave = i - lane + 64 <= N;
     const bool wave_any = __ballot(any) != 0;
@@ -353,6 +353,7 @@ __global__ __launch_bounds__(256, GS_K8_WAVES) void param_bwd_kernel(
 #pragma unroll
         for (int vv = 0; vv < 12; vv++)
             s_sh4[vv][threadIdx.x] = make_float4(acc_sh[4 * vv], acc_sh[4 * vv + 1], acc_sh[4 * vv + 2], acc_sh[4 * vv + 3]);
+        wave_lds_fence();
         float4 *dst = reinterpret_cast<float4 *>(dL_dsh + (size_t)(i - lane) * 48);
         const int col0 = threadIdx.x - lane;
 #pragma unroll

@@ -334,7 +334,7 @@ __global__ __launch_bounds__(256) GS_K1_OCC void preprocess_batch_kernel(int N, 
             float4 geo, con, rgb;
             gs_make_record(o.cx, o.cy, opac, o.con[0], o.con[1], o.con[2], o.col[0], o.col[1], o.col[2], geo, con, rgb);
             // The wave's 64 records go through wave-private LDS ([quarter][lane], pitch 68 float4: conflict-free both
-            // ways; one wave's LDS operations execute in order, so no barrier) and leave as four stores of 1 KiB of
+            // ways; a fence of the wave on either side of the reads, no barrier) and leave as four stores of 1 KiB of
             // whole lines each, instead of four stores of 64 quarter lines: 0.228 -> 0.202 ms per 8 views.  (Leaving
             // the unused fourth quarter unwritten costs a read-modify-write per line: 0.303 ms.)
             __shared__ float4 s_rec[4][4][68];
@@ -345,7 +345,9 @@ __global__ __launch_bounds__(256) GS_K1_OCC void preprocess_batch_kernel(int N, 
             const float4 rq = make_float4(__int_as_float(o.rect[0]), __int_as_float(o.rect[1]), __int_as_float(o.rect[2]),
                                             __int_as_float(o.rect[3]));
             if (i - lane + 64 <= N) {
+                wave_lds_fence();                      // the previous view's records have been read
                 st[0][lane] = geo; st[1][lane] = con; st[2][lane] = rgb; st[3][lane] = rq;
+                wave_lds_fence();
                 float4 *dst = w.records + (size_t)(i - lane) * 4;
 #pragma unroll
                 for (int k = 0; k < 4; k++) {

@@ -27,9 +27,9 @@ def _device_code(source):
         elif events is not None:
             if re.search(r"amdgcn\.(wave|s)\.barrier\(", line):
                 events.append("F")
-            elif re.match(r"\s+store .* addrspace\(3\)", line):
+            elif re.match(r"\s+store .* addrspace\(3\)|.* @llvm\.memcpy\.p3\.", line):
                 events.append("S")
-            elif re.match(r"\s+%\S+ = load .* addrspace\(3\)", line):
+            elif re.match(r"\s+%\S+ = load .* addrspace\(3\)|.* @llvm\.memcpy\.p\d+\.p3\.", line):
                 events.append("L")
     return {k: re.sub(r"(.)\1+", r"\1", "".join(e)) for k, e in kernels.items()}
 
@@ -39,3 +39,18 @@ def test_rows_of_packed_sh_leave_between_fences():
     assert len(found) == 1 + 1 + 8                       # quantise; dequantise; gradients of four degrees, few and several views
     for kernel, events in found.items():
         assert "SL" not in events and "LS" not in events, (kernel, events)
+
+
+def test_view_records_leave_between_fences():
+    found = {k: e for k, e in _device_code("preprocess.hip").items() if "S" in e}
+    assert len(found) == 8                               # records: fast and general, packed or not, opacities per view or not
+    for kernel, events in found.items():
+        assert "SL" not in events and "LS" not in events, (kernel, events)
+        assert events.startswith("F"), (kernel, events)  # the loop over the views comes back to the stores
+
+
+def test_parameter_gradients_leave_behind_a_fence():
+    found = {k: e for k, e in _device_code("param_bwd.hip").items() if "S" in e}
+    assert len(found) == 8
+    for kernel, events in found.items():                 # in front: a thread's own column, written and read by itself alone
+        assert re.fullmatch(r"(SL)+SFL", events), (kernel, events)

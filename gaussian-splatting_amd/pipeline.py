@@ -74,12 +74,37 @@ class View:
         self.camera, self.camera_r, self.camera_t = camera, camera_r, camera_t
 
 
+class _KeptRecords:
+    """The packed SH that a K1 launch read, kept with the views it made: their K8 reads the same records, whatever `sh` has
+    been packed to since and on whichever stream."""
+
+    def __init__(self, packed, ctx=None):
+        self.packed = packed
+        # packed on ctx's current stream by what has just been launched; None: the caller's own records
+        self.stream = ctx.current_stream() if ctx is not None else None
+        self.ready = self.stream.record_event() if self.stream is not None and not self._captured() else None
+
+    def _captured(self):
+        """In a captured graph the capture itself orders what is launched."""
+        return self.packed.words.is_cuda and torch.cuda.is_current_stream_capturing()
+
+    def on(self, ctx):
+        """The records, for a launch on ctx's current stream."""
+        if self.ready is not None and not self._captured():
+            stream = ctx.current_stream()
+            if stream != self.stream:
+                stream.wait_event(self.ready)
+                if self.packed.words.is_cuda:
+                    self.packed.words.record_stream(stream)
+        return self.packed
+
+
 class SplatPipeline:
     """Holds the parameters on one device and runs views through the native kernels.
 
     sh_format="mxfp4": views are rendered from packed SH (32-byte records, gs_sh_quantize).  The coefficients in `sh` stay
-    the parameters: every K1 launch packs them as they are then (`packed`), and the gradients K8 forms with respect to the
-    packed values are taken for theirs, so that a scene trained this way looks the same when it is served from its records.
+    the parameters: every K1 launch packs them as they are then (`packed`; a view's state keeps the records it was
+    rendered from), and the gradients K8 forms with respect to the packed values are taken for theirs, so that a scene trained this way looks the same when it is served from its records.
     A gaussian set whose spherical_harmonics are a PackedSH is served from those: `sh` is None, and there is nothing to
     train."""
 
@@ -91,6 +116,7 @@ class SplatPipeline:
         dev = self.ctx.device
         self.N, self.means, self.log_scales, self.quats, self.sh = api._gaussian_tensors(gaussians, dev)
         self.packed = None
+        self._packed_kept = None
         if api._is_packed(self.sh):
             self.packed, self.sh = self.sh, None
         if sh_format not in (None, "fp32", "mxfp4"):
@@ -157,16 +183,28 @@ class SplatPipeline:
             sh = f(self.packed.dequantize(self.ctx) if self.sh is None else self.sh)
         return api.GaussianSet(f(self.means), sh, f(self.log_scales), f(self.quats), f(self.opacity), self.degrees)
 
+    def _kept(self):
+        """What a view's state keeps of the SH coefficients: the records last packed, or None without any."""
+        if self.packed is None:
+            return None
+        if self._packed_kept is None or self._packed_kept.packed is not self.packed:
+            self._packed_kept = _KeptRecords(self.packed)
+        return self._packed_kept
+
     def _kept_sh(self, c):
         """pack_sh without packing again what the last K1 launch packed."""
-        return self.packed if self.packed is not None and len(self.packed) == self.N else self.pack_sh(c)
+        if self.packed is not None and len(self.packed) == self.N:
+            return self._kept().on(c)
+        return self.pack_sh(c)
 
     def pack_sh(self, ctx=None):
         """What K1 and K8 take the SH coefficients from: `sh`, or with sh_format "mxfp4" its records, packed here."""
         if self.sh_format != "mxfp4":
             return self.sh
         if self.sh is not None:
-            self.packed = quantize_sh(self.sh, ctx=ctx or self.ctx)
+            c = ctx or self.ctx
+            self.packed = quantize_sh(self.sh, ctx=c)
+            self._packed_kept = _KeptRecords(self.packed, c)
         return self.packed
 
     # ---- forward ------------------------------------------------------------------------
@@ -221,7 +259,7 @@ class SplatPipeline:
                 else:
                     check(c.lib.gs_preprocess_batch_records_views(*args, self.N, len(pres), arr),
                           "gs_preprocess_batch_records_views")
-            return self._with_dropout(pres, dropout)
+            return self._kept_with(pres, dropout)
         pres = [self._alloc_pre(cam) for cam in cams]
         arr = (GsViewPreprocess * max(len(pres), 1))()
         for k, p in enumerate(pres):
@@ -234,12 +272,13 @@ class SplatPipeline:
                                             api._ptr(self.quats), sh_ptr, len(pres), arr), "gs_preprocess_batch")
         for k, p in enumerate(pres):
             p["opac"] = view_opac(k)
-        return self._with_dropout(pres, dropout)
+        return self._kept_with(pres, dropout)
 
-    @staticmethod
-    def _with_dropout(pres, dropout):
-        if dropout is not None:
-            for p in pres:
+    def _kept_with(self, pres, dropout):
+        """What K8 needs of the launch that made these views."""
+        for p in pres:
+            p["packed"] = self._kept()
+            if dropout is not None:
                 p["opacity_scale"] = dropout.scale
         return pres
 
@@ -262,6 +301,7 @@ class SplatPipeline:
                                           api._ptr(pre["centers"]), api._ptr(pre["depths"]), api._ptr(pre["colors"]),
                                           api._ptr(pre["conics"]), api._ptr(pre["clamped"]), api._ptr(pre["rect"]),
                                           api._ptr(pre["radii"]), null, null, null, null, null, null), "gs_preprocess")
+            pre["packed"] = self._kept()
         opac = pre.get("opac")
         if opac is None:
             opac = torch.sigmoid(self.opacity) if self.opacity_is_logit else self.opacity
@@ -307,7 +347,7 @@ class SplatPipeline:
         c.sync_stream()
         state = dict(ctx=c, cam=pre["cam"], depths=pre["depths"], centers=pre["centers"], colors=pre["colors"],
                      conics=pre["conics"], clamped=pre["clamped"], radii=pre["radii"], opac=opac, binning=binning,
-                     rec=pre.get("rec"), opacity_scale=pre.get("opacity_scale"))
+                     rec=pre.get("rec"), opacity_scale=pre.get("opacity_scale"), packed=pre.get("packed"))
         with _records(c, self.N, pre.get("rec")):
             if loss is None:
                 image, n_contrib, t_final = api.blend_forward(c, pre["centers"], pre["colors"], opac, pre["conics"],
@@ -365,12 +405,32 @@ class SplatPipeline:
         parameters are read once and the gradients written (or added) once.  g_range=(g0, g1) restricts
         the launch to those gaussians (every array of the call is per-gaussian and contiguous, so a range
         is the same call on offset pointers); g0 must be a multiple of 4 (16-byte aligned rows of every
-        array)."""
+        array).  Views that were rendered from different packed SH (sh_format "mxfp4", K1 launches that packed anew) take a
+        launch for each."""
         c = ctx or self.ctx
         c.sync_stream()
         g0, g1 = (0, self.N) if g_range is None else (int(g_range[0]), int(g_range[1]))
         if not (0 <= g0 <= g1 <= self.N) or g0 % 4:
             raise ValueError(f"g_range {g_range} must lie in [0, {self.N}] and start at a multiple of 4")
+        for st in states:
+            if st["radii"].shape[0] != self.N:
+                raise ValueError(f"the view was rendered with {st['radii'].shape[0]} gaussians, the pipeline has {self.N}")
+        groups = []      # (records, the states rendered from them), in the order of the states
+        for st in states:
+            kept = st.get("packed")
+            for k, members in groups:
+                if k is kept:
+                    members.append(st)
+                    break
+            else:
+                groups.append((kept, [st]))
+        for kept, members in groups or [(None, [])]:
+            sh = self._kept_sh(c) if kept is None else kept.on(c)
+            self._backward_params(c, members, sh, grads, accumulate, g0, g1)
+            accumulate = True
+        return grads
+
+    def _backward_params(self, c, states, sh, grads, accumulate, g0, g1):
         at = lambda t, width: ctypes.c_void_p(t.data_ptr() + g0 * width * t.element_size())
         views = (GsViewBackward * max(len(states), 1))()
         for k, st in enumerate(states):
@@ -378,7 +438,7 @@ class SplatPipeline:
             views[k].radii = at(st["radii"], 1).value
             views[k].clamped = at(st["clamped"], 3).value
             views[k].grad_rows = at(st["rows"], 16).value
-        with api.bound_sh(c, g1 - g0, self._kept_sh(c), first=g0) as sh_ptr:
+        with api.bound_sh(c, g1 - g0, sh, first=g0) as sh_ptr:
             head = (c.handle, g1 - g0, at(self.means, 3), at(self.log_scales, 3), at(self.quats, 4), sh_ptr,
                     at(self.opacity, 1), int(self.opacity_is_logit), len(states), views)
             tail = (int(bool(accumulate)), at(grads.means, 3), at(grads.log_scales, 3), at(grads.quats, 4),
@@ -388,7 +448,6 @@ class SplatPipeline:
             else:      # views blended with dropped-out opacities
                 scale = (ctypes.c_float * len(states))(*[st.get("opacity_scale") or 1.0 for st in states])
                 check(c.lib.gs_backward_params_batch_scaled(*head, scale, *tail), "gs_backward_params_batch_scaled")
-        return grads
 
     def backward(self, state, dL_dimage, grads, accumulate=True):
         """d(loss)/d(parameters) of one view into `grads` (FlatGrads), added when accumulate."""

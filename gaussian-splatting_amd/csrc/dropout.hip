@@ -64,6 +64,13 @@ __device__ __forceinline__ void last_round(const State &s, uint64_t seed, uint32
 
 __device__ __forceinline__ float activated(float x, int is_logit) { return is_logit ? 1.0f / (1.0f + expf(-x)) : x; }
 
+// sigmoid'(x) = e / (1 + e)^2 with e = exp(-|x|): six roundings at every x.  (o (1 - o) cancels where o is close to 1: 1 % off
+// at x = 12, exactly 0 from 17.4 on, where the value is 2.8e-8.)
+__device__ __forceinline__ float sigmoid_derivative(float x) {
+    const float e = expf(-fabsf(x)), d = 1.0f + e;
+    return e / (d * d);
+}
+
 // PER neighbouring gaussians per thread, loaded and stored together; rows of N floats start at any multiple of 4 bytes.
 // `all` is uniform in a block: the last block of a launch goes element by element.
 template <int PER>
@@ -181,10 +188,7 @@ __global__ __launch_bounds__(256) void opacity_dropout_backward_kernel(int N, co
     if (is_logit) {
         r.load(opacity + i, all, n);
 #pragma unroll
-        for (int e = 0; e < PER; e++) {
-            const float o = activated(r.v[e], 1);
-            sum.v[e] *= o * (1.0f - o);
-        }
+        for (int e = 0; e < PER; e++) sum.v[e] *= sigmoid_derivative(r.v[e]);
     }
     if (accumulate) r.load(d_opacity + i, all, n);
 #pragma unroll

@@ -334,9 +334,11 @@ __global__ __launch_bounds__(256, GS_K8_WAVES) void param_bwd_kernel(
             g_q[2] = s * py - k2 * qy;
             g_q[3] = s * pz - k2 * qz;
         }
-        if (ROWS && opacity && opacity_is_logit) {     // opacity = sigmoid(parameter)
-            const float o = 1.0f / (1.0f + __expf(-opacity[i]));
-            g_op *= o * (1.0f - o);
+        if (ROWS && opacity && opacity_is_logit) {
+            // opacity = sigmoid(parameter): its derivative as e / (1 + e)^2, e = exp(-|x|), which does not cancel where the
+            // opacity is close to 1 (o (1 - o) is 0 from x = 17.4 on)
+            const float e = __expf(-fabsf(opacity[i])), d = 1.0f + e;
+            g_op *= e / (d * d);
         }
     }
 

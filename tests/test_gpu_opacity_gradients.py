@@ -35,3 +35,38 @@ def test_dropout_gradient_of_confident_gaussians(gpu_ctx, n, p, views):
     tol = np.abs(s).sum(axis=0) * act / (1 - p) * (9 + len(views)) * U
     assert (np.abs(got - s.sum(axis=0) * act / (1 - p)) <= tol).all()
     assert (got[:2 * len(FAR)][keep.all(axis=0)[:2 * len(FAR)]] != 0).all()
+
+
+@pytest.mark.parametrize("general", [False, True])
+def test_parameter_backward_of_confident_gaussians(gpu_ctx, general, monkeypatch):
+    """K8 on logits against K8 on the opacities they stand for: the same images and rows, times the derivative."""
+    import torch
+    import gsplat_amd as gs
+    from test_gpu_packed_train import _scene, _targets, _views, _with
+    if general:
+        monkeypatch.setenv("GS_K8_GENERAL", "1")
+    c = gpu_ctx.clone()
+    c.set_option("deterministic_backward", 1)
+    cam, g, rs = _scene(1501)
+    x = np.random.default_rng(2).choice([2.0, 7.5] + FAR, size=1501).astype(np.float32)
+    views, targets = _views(gs, cam, 3), _targets(c, rs, 3)
+    logits = gs.SplatPipeline(_with(g, opacity=x), rs, ctx=c)
+    raw = gs.SplatPipeline(_with(g, opacity=torch.sigmoid(logits.opacity)), rs, ctx=c, opacity_is_logit=False)
+    grads = []
+    for pipe in (logits, raw):
+        gr = gs.FlatGrads(pipe.N, c.device)
+        gs.train_step(pipe, views, targets, gr, concurrent_views=1)
+        torch.cuda.synchronize()
+        grads.append(gr)
+    assert torch.equal(grads[0].means, grads[1].means)
+    got, by_opacity = (gr.opacity.double().cpu().numpy() for gr in grads)
+    e = np.exp(-np.abs(x.astype(np.float64)))
+    want = by_opacity * e / (1 + e) ** 2
+    # exp as 2^(x log2 e): the product and its constant are each off by u, which x turns into 2 |x| u of the result, and one
+    # step (2 u) of the hardware's exp2; then four roundings of 1 + e, the square and the quotient, and the product.  The
+    # products at x = 80 (1.8e-35 times gradients down to 1e-12) leave fp32's normal numbers: there the last rounding is off
+    # by half of their spacing 2^-149 whatever the value, which is 2^-150
+    assert (np.abs(got - want) <= (2 * np.abs(x) + 8) * U * np.abs(want) + 2.0 ** -150).all()
+    far = (x >= 17) & (np.abs(want) >= 2.0 ** -126)
+    assert far.sum() > 100 and (got[far] != 0).all()
+    c.close()

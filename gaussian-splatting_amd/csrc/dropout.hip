@@ -157,6 +157,7 @@ __global__ __launch_bounds__(256) void opacity_dropout_backward_kernel(int N, co
     const bool all = (blockIdx.x + 1) * (256u * PER) <= (uint32_t)N;
     const uint32_t n = min((uint32_t)PER, (uint32_t)N - i);
     Row<PER> sum = {};
+    bool kept[PER] = {};                                // by one of the views
 #pragma unroll 1
     for (int g = 0; g < groups.n; g++) {
         const ViewGroup group = groups.g[g];
@@ -172,7 +173,8 @@ __global__ __launch_bounds__(256) void opacity_dropout_backward_kernel(int N, co
         for (int e = 0; e < PER; e++) s[e] = nine_rounds(i + e, group.block, seed);
 #pragma unroll
         for (int pair = 0; pair < 2; pair++) {
-            if (group.view(2 * pair) == NO_VIEW && group.view(2 * pair + 1) == NO_VIEW) continue;
+            const bool has0 = group.view(2 * pair) != NO_VIEW, has1 = group.view(2 * pair + 1) != NO_VIEW;
+            if (!has0 && !has1) continue;
 #pragma unroll
             for (int e = 0; e < PER; e++) {
                 uint32_t w0, w1;
@@ -181,6 +183,7 @@ __global__ __launch_bounds__(256) void opacity_dropout_backward_kernel(int N, co
                 // selected: a NaN of a dropped gaussian stays out
                 sum.v[e] += w0 >= limit ? d[2 * pair].v[e] : 0.0f;
                 sum.v[e] += w1 >= limit ? d[2 * pair + 1].v[e] : 0.0f;
+                kept[e] |= (has0 && w0 >= limit) || (has1 && w1 >= limit);
             }
         }
     }
@@ -188,7 +191,7 @@ __global__ __launch_bounds__(256) void opacity_dropout_backward_kernel(int N, co
     if (is_logit) {
         r.load(opacity + i, all, n);
 #pragma unroll
-        for (int e = 0; e < PER; e++) sum.v[e] *= sigmoid_derivative(r.v[e]);
+        for (int e = 0; e < PER; e++) sum.v[e] = kept[e] ? sum.v[e] * sigmoid_derivative(r.v[e]) : 0.0f;      // 0 times a NaN
     }
     if (accumulate) r.load(d_opacity + i, all, n);
 #pragma unroll

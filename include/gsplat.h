@@ -476,7 +476,8 @@ int gs_backward_params_batch_scaled(gs_ctx *ctx, int32_t N, const float *means, 
  * word (s & 3) of Philox4x32-10 at the counter (i, 0, low and high 32 bits of s >> 2) under the key `seed` is at least
  * round(p 2^32), 0 <= p < 1.  gs_opacity_dropout_backward evaluates it again:
  * dL_dopacity[i] = do/dopacity / (1 - p) * sum over the views that keep i of dL_dout[view][i], written, or added to when
- * accumulate != 0; gradients of left-out gaussians are not read into the sum, NaN included. */
+ * accumulate != 0; gradients of left-out gaussians are not read into the sum, NaN included, and a gaussian that every view
+ * leaves out gets 0, whatever its opacity is. */
 int gs_opacity_dropout(gs_ctx *ctx, int32_t N, const float *opacity, int32_t opacity_is_logit, double p, uint64_t seed,
                        int32_t n_views, const uint64_t *view_ids_host, float *out);
 int gs_opacity_dropout_backward(gs_ctx *ctx, int32_t N, const float *opacity, int32_t opacity_is_logit, double p,

@@ -70,3 +70,32 @@ def test_parameter_backward_of_confident_gaussians(gpu_ctx, general, monkeypatch
     far = (x >= 17) & (np.abs(want) >= 2.0 ** -126)
     assert far.sum() > 100 and (got[far] != 0).all()
     c.close()
+
+
+@pytest.mark.parametrize("n", [180, (1 << 19) + 90])
+@pytest.mark.parametrize("is_logit", [False, True])
+def test_dropout_gradient_of_gaussians_left_out_of_every_view(gpu_ctx, n, is_logit):
+    """0 whatever the opacity is, as their opacities are in the forward pass; the others get the formula's value."""
+    import torch
+    import gsplat_amd as gs
+    d = gpu_ctx.device
+    some = torch.tensor([float("nan"), float("inf"), -float("inf"), 1e30, -1e30, 0.0, -0.0, 200.0, -200.0], device=d)
+    x = some.repeat((n + 8) // 9)[:n].contiguous()
+    for views in ([4], [0, 1, 2], [3, 8, 13, 18], list(range(0, 5 * 40, 5)), []):       # 40 blocks: two launches
+        p = .5 if len(views) < 10 else .97
+        keep = gs.dropout_opacity(torch.ones_like(x), p, 7, views, ctx=gpu_ctx) != 0
+        some_view = keep.any(dim=0) if views else torch.zeros(n, dtype=torch.bool, device=d)
+        assert not views or 0 < int(some_view.sum()) < n
+        got = gs.dropout_opacity_backward(torch.ones((len(views), n), device=d), x, p, 7, views, is_logit=is_logit, ctx=gpu_ctx)
+        assert (got[~some_view] == 0).all()
+        act = torch.ones(n, dtype=torch.float64, device=d)
+        if is_logit:
+            act = torch.where(x == 0, .25, 0.0).double()
+            act[x.isnan()] = float("nan")
+        want = (keep.sum(dim=0) * act / (1 - p))[some_view]
+        # counts and 1/4 are exact: the scale's rounding and the product, per launch, and the launches' sum
+        torch.testing.assert_close(got[some_view].double(), want, rtol=6 * U, atol=0, equal_nan=True)
+        out = torch.full((n,), 2.0, device=d)
+        gs.dropout_opacity_backward(torch.ones((len(views), n), device=d), x, p, 7, views, is_logit=is_logit, ctx=gpu_ctx,
+                                    out=out, accumulate=True)
+        assert (out[~some_view] == 2).all()

@@ -185,7 +185,7 @@ class SplatPipeline:
 
     def _kept(self):
         """What a view's state keeps of the SH coefficients: the records last packed, or None without any."""
-        if self.packed is None:
+        if self.packed is None or self.sh_format != "mxfp4":
             return None
         if self._packed_kept is None or self._packed_kept.packed is not self.packed:
             self._packed_kept = _KeptRecords(self.packed)
@@ -193,9 +193,8 @@ class SplatPipeline:
 
     def _kept_sh(self, c):
         """pack_sh without packing again what the last K1 launch packed."""
-        if self.packed is not None and len(self.packed) == self.N:
-            return self._kept().on(c)
-        return self.pack_sh(c)
+        kept = self._kept()
+        return kept.on(c) if kept is not None and len(kept.packed) == self.N else self.pack_sh(c)
 
     def pack_sh(self, ctx=None):
         """What K1 and K8 take the SH coefficients from: `sh`, or with sh_format "mxfp4" its records, packed here."""

@@ -124,3 +124,57 @@ def test_dropout_on_the_exact_lists(det_ctx, lanes):      # noqa: F811
         assert (gv.means[dropped[v] == 0] == 0).all() and (gv.sh[dropped[v] == 0] == 0).all()
         want = want + gv.sh.double()
     assert float((b.sh.double() - want).abs().max()) <= 2 ** -18 * float(want.abs().max())
+
+
+def test_captured_between_eager_launches(det_ctx):      # noqa: F811
+    """K1 with its packing, and K8 of views that were rendered before, in a graph on another stream: each replay reads the
+    coefficients and rows as they are then, and eager launches go on around it."""
+    import torch
+    import gsplat_amd as gs
+    cam, g, rs = _scene(1003)
+    views, targets = _views(gs, cam, 3), _targets(det_ctx, rs, 3)
+    pipe = gs.SplatPipeline(g, rs, ctx=det_ctx, sh_format="mxfp4")
+
+    def rendered():
+        states = []
+        for k, pre in enumerate(pipe.preprocess_batch(views)):
+            image, st = pipe.forward(views[k], pre=pre)
+            pipe.backward_rows(st, pipe.image_loss(image, targets[k], "l2")[0])
+            states.append(st)
+        return states
+
+    states = rendered()
+    out = gs.FlatGrads(pipe.N, det_ctx.device)
+    side = det_ctx.new_stream()
+    side.wait_stream(det_ctx.current_stream())
+    with det_ctx.use_stream(side):
+        pipe.backward_params(states, out)
+        pipe.preprocess_batch(views)
+    det_ctx.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pres = pipe.preprocess_batch(views)
+        pipe.backward_params(states, out)
+    captured = pres[0]["packed"]
+    assert captured is not states[0]["packed"]
+    sh = pipe.sh.clone()
+    for scale in (1.0, 0.5, -2.0):
+        pipe.sh.copy_(scale * sh)
+        for st in states:
+            st["rows"].mul_(scale)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = gs.FlatGrads(pipe.N, det_ctx.device)
+        pipe.backward_params(states, want)
+        for a, b in zip(pres, pipe.preprocess_batch(views)):
+            assert torch.equal(a["rec"], b["rec"]) and torch.equal(a["clamped"], b["clamped"])
+        assert torch.equal(out.flat, want.flat) and float(want.flat.abs().max()) > 0
+        torch.cuda.synchronize()
+    # the records packed inside the graph serve an eager launch too
+    same = gs.FlatGrads(pipe.N, det_ctx.device)
+    pipe.backward_params([dict(st, packed=captured) for st in states], same)
+    fresh = [dict(st, packed=pre["packed"]) for st, pre in zip(states, pipe.preprocess_batch(views))]
+    want = gs.FlatGrads(pipe.N, det_ctx.device)
+    pipe.backward_params(fresh, want)
+    torch.cuda.synchronize()
+    assert torch.equal(same.flat, want.flat)

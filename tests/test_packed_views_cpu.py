@@ -143,3 +143,12 @@ def test_records_given_as_parameters_stay_the_callers():
     state = _render(pipe, views[0])
     pipe.backward_params([state], gs.FlatGrads(N, torch.device("cpu")))
     assert lib.packings == 1 and lib.read == [(1, 1, 0)] and ctx.stream.waited == [] and ctx.stream.recorded == []
+
+
+def test_a_pipeline_set_back_to_its_coefficients_reads_them():
+    gs, lib, ctx, pipe = _pipe()
+    views, _ = _views_targets(gs, 1)
+    _render(pipe, views[0])
+    pipe.sh_format = "fp32"
+    pre = pipe.preprocess_batch(views, repack=False)[0]
+    assert pre["packed"] is None and pipe._kept_sh(ctx) is pipe.sh

@@ -8,8 +8,9 @@
 //
 // They have to move 4 + 4 V bytes per gaussian forward, 8 + 4 V backward, and to evaluate the generator once per gaussian
 // and block of four view numbers -- once per view for the views a rank of a multi-rank job renders, whose numbers lie apart.
-// That evaluation, some 70 instructions, bounds them: 10 M gaussians x 4 views of different blocks 57 us = 3.5 TB/s, the
-// gradient 60 us; 1 M x 8 views 17.8 us.
+// That evaluation, some 70 instructions, bounds them where every view needs its own: 10 M gaussians x 4 views 56 us = 3.6
+// TB/s, the gradient 61 us; 1 M x 8 views 15 us and 16 us.  Consecutive view numbers, as a training on one GPU counts them,
+// share evaluations and come to the memory's rate: 35 us = 5.7 TB/s and 44 us = 5.5 TB/s; 9.6 us and 10.5 us.
 #include "common.h"
 #include <math.h>
 #include <string.h>
@@ -200,8 +201,9 @@ __global__ __launch_bounds__(256) void opacity_dropout_backward_kernel(int N, co
 }
 
 // Gaussians per thread: four share a view's scalar work and store 16 bytes at once, but leave small scenes with few waves.
-// us forward / backward with one and with four: 10 k x 8 views 7.3 / 7.3 and 9.2 / 9.6, 300 k x 8 9.7 / 9.3 and 11.7 / 11.5,
-// 1 M x 8 18.2 / 17.8 and 17.8 / 17.2, 10 M x 4 63 / 69 and 57 / 60.
+// us forward / backward of the kernels with one and with four (profiler, fastest launches): 10 k x 8 views 4.4 / 5.1 and
+// 6.9 / 8.4, 300 k x 8 7.2 / 7.8 and 9.2 / 9.0, 524 k x 8 9.0 / 10.0 and 9.9 / 10.7, 1 M x 8 14.3 / 15.1 and 14.1 / 15.1,
+// 10 M x 4 64 / 82 and 54 / 61.
 inline int per_thread(int32_t N) { return N >= (1 << 19) ? 4 : 1; }
 
 int check_dropout(const char *who, gs_ctx *ctx, int32_t N, double p, int32_t n_views, const uint64_t *view_ids, uint32_t *limit,

@@ -312,7 +312,8 @@ __global__ __launch_bounds__(256) GS_K1_OCC void preprocess_batch_kernel(int N, 
     load_params<PACKED>(i, means, log_scales, quats, sh, x, y, z, q, ls, coef);
     const float opac0 = RECORDS ? opacities[i] : 0.0f;
     // (VIEW_OPACITIES: opacities of its own per view, opacity_stride apart.  A template argument: what a record holds of the
-    // opacity is formed once for all views otherwise, 235 against 258 us per 8 views)
+    // opacity is formed once for all views otherwise, 235 against 258 us per 8 views when alone; in a step of 1 M gaussians
+    // now 195 us, and 230 with opacities per view)
     // M and Sigma once per gaussian: the host has checked that the views share scale_mod and the scale switch
     double M[9], Sg[9];
     gaussian_cov(b.cam[0].scale_mod, b.cam[0].diag_scale, q[0], q[1], q[2], q[3], ls, M, Sg);

@@ -79,8 +79,9 @@ __device__ __forceinline__ void registers_to_rows(Columns<ROUNDS> &s, const Rows
 }
 
 // A thread per channel: its 64 bytes in four loads.  The three threads of a gaussian, which may sit in different waves, meet
-// in LDS, and the records leave 16 bytes per thread.  1 M gaussians 40 us = 5.6 TB/s, 5 M 205 us (a thread per gaussian,
-// twelve loads 192 bytes apart: 43 and 208; non-temporal loads drop the lines between them: 100 and 487).
+// in LDS, and the records leave 16 bytes per thread.  5 M gaussians 200 us = 5.6 TB/s.  (1 M and 5 M when this was chosen: 40
+// and 205 us; a thread per gaussian, twelve loads 192 bytes apart: 43 and 208; non-temporal loads drop the lines between
+// them: 100 and 487.)
 constexpr int QUANT_GAUSSIANS = 64;
 __global__ __launch_bounds__(3 * QUANT_GAUSSIANS) void sh_quantize_kernel(int N, const float4 *__restrict__ sh,
                                                                           uint4 *__restrict__ words) {
@@ -112,7 +113,7 @@ __global__ __launch_bounds__(3 * QUANT_GAUSSIANS) void sh_quantize_kernel(int N,
                         : make_uint4(r.w | g.w << 16, b.w | r.z << 16 | g.z << 24, r.x, r.y | b.z << 28);
 }
 
-// 1 M gaussians 35 us, 5 M 178 us = 6.3 TB/s.
+// 5 M gaussians 175 us = 6.4 TB/s.
 __global__ __launch_bounds__(256) void sh_dequantize_kernel(int N, const uint4 *__restrict__ words, float4 *__restrict__ sh) {
     __shared__ Columns<1> s_col;
     const uint32_t i = blockIdx.x * 256u + threadIdx.x;
@@ -201,8 +202,9 @@ __device__ __forceinline__ double evaluate(const Polynomial &p, double x, double
 
 // In fp64 from the difference of the positions on, as K1 evaluates colours: the flag is the sign of the sum.
 // SEVERAL views are bound by the fp64 arithmetic of the view loop, and turning the coefficients into a Polynomial in front of
-// it pays: 1 M gaussians x 8 views 36 us = 4.6 TB/s (42 without), 3 M x 4 views 64 (67).  A single view does not earn that
-// back and stays at the memory's rate without: 10 M gaussians 103 us = 5.7 TB/s (117 with).
+// it pays: 1 M gaussians x 8 views 33 us = 5.0 TB/s (39 without), 3 M x 4 views 59 (63).  Two views are even (1 M 15 us either
+// way, 5 M 68 with, 64 without).  A single view does not earn it back and stays at the memory's rate without: 10 M gaussians
+// 104 us (119 with; fastest launches, both sides under the profiler: outside it a call takes 96 us = 6.1 TB/s).
 template <int DEGREE, bool SEVERAL>
 __global__ __launch_bounds__(256, 4) void sh_color_kernel(int N, const uint4 *__restrict__ words, const float *__restrict__ means,
                                                           const Cameras cams, float *__restrict__ colors,
@@ -243,10 +245,10 @@ __global__ __launch_bounds__(256, 4) void sh_color_kernel(int N, const uint4 *__
 
 // fp32 behind the fp64 direction, as in K8: products and sums of a few dozen terms.  The constants of the basis are taken
 // out of the sums: they are multiplied in behind the view loop.
-// Few views are bound by the rows that are written: the coefficients are decoded once (10 M gaussians x 1 view 427 us = 6.2
+// Few views are bound by the rows that are written: the coefficients are decoded once (10 M gaussians x 1 view 425 us = 6.2
 // TB/s).  SEVERAL views are bound by the loop's loads and its 200 vector instructions, and gain more by a fourth wave per SIMD
 // than they lose by decoding the record in every view (45 registers less) and storing in two rounds: 1 M x 8 views 77 us
-// against 85, 3 M x 4 168 against 176; 10 M x 1 466 against 427, 1 M x 2 the same.
+// against 85, 3 M x 4 163 against 170, 1 M x 3 52 against 53; 10 M x 1 438 against 417, two views the same (1 M 42, 5 M 230).
 template <int DEGREE, bool SEVERAL>
 __global__ __launch_bounds__(256, SEVERAL ? 4 : 1) void sh_color_backward_kernel(
     int N, const uint4 *__restrict__ words, const float *__restrict__ means, const Cameras cams,

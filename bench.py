@@ -34,10 +34,10 @@ if ROOT not in sys.path:
     sys.path.insert(0, ROOT)
 
 HBM_PEAK_GBS = 8000.0     # MI355X_MICROARCH.md: HBM3E 8 TB/s spec
-PMC_SUMMARY = "r03_pmc_summary.json"
+PMC_SUMMARY = "pmc_summary.json"
 # counter summaries of other workloads (tools/pmc_collect.sh with GS_N / GS_W / GS_H / GS_LS* / GS_LISTS): the one whose
 # source hash and workload match the run is used
-PMC_SUMMARIES = (PMC_SUMMARY, "r03_pmc_summary_culled.json", "r03_pmc_summary_10m4k.json")
+PMC_SUMMARIES = (PMC_SUMMARY, "pmc_summary_culled.json", "pmc_summary_10m4k.json")
 # stages whose launch is several kernels: the counters of the stage are the sums over its parts
 PMC_PARTS = {"bin_sort": ("tile_hist", "tile_hist2", "tile_scatter")}     # (+ the 256-block scans, not separable by name)
 LISTS_NOTE = {

@@ -463,7 +463,8 @@ int gs_preprocess_batch_records_views(gs_ctx *ctx, int32_t N, const float *means
 
 /* gs_backward_params_batch for views that were blended with dropped-out opacities: the opacity gradient of view v is
  * multiplied by opacity_scale_host[v] (HOST, 1 / (1 - p); NULL: 1 for every view).  That is the whole backward pass of the
- * dropout: a gaussian that was left out has opacity 0, reaches alpha 1/255 nowhere, and its gradient row is zero. */
+ * dropout: a gaussian that was left out has opacity 0, reaches alpha 1/255 nowhere, and its gradient row is zero.  (A NaN
+ * logit has a NaN derivative here, as without dropout: 0 times it is NaN.) */
 int gs_backward_params_batch_scaled(gs_ctx *ctx, int32_t N, const float *means, const float *log_scales,
                                     const float *quats, const float *sh, const float *opacity,
                                     int32_t opacity_is_logit, int32_t n_views, const gs_view_backward *views,

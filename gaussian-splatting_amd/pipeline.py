@@ -103,10 +103,10 @@ class SplatPipeline:
     """Holds the parameters on one device and runs views through the native kernels.
 
     sh_format="mxfp4": views are rendered from packed SH (32-byte records, gs_sh_quantize).  The coefficients in `sh` stay
-    the parameters: every K1 launch packs them as they are then (`packed`; a view's state keeps the records it was
-    rendered from), and the gradients K8 forms with respect to the packed values are taken for theirs, so that a scene trained this way looks the same when it is served from its records.
-    A gaussian set whose spherical_harmonics are a PackedSH is served from those: `sh` is None, and there is nothing to
-    train."""
+    the parameters: every K1 launch packs them as they are then (`packed`; a view's state keeps the records it was rendered
+    from), and the gradients K8 forms with respect to the packed values are taken for theirs, so that a scene trained this
+    way looks the same when it is served from its records.  A gaussian set whose spherical_harmonics are a PackedSH is
+    served from those: `sh` is None, and there is nothing to train."""
 
     def __init__(self, gaussians, result_size, tile_size=16, background=(0., 0., 0.), pixel_offset=0.5,
                  opacity_is_logit=True, ctx=None, cull_tiles=True, apply_view=False, diag_scale=False, sh_format=None):
